@@ -84,6 +84,79 @@ B200_API int32_t b200_store_kvcache(const void* key, int64_t key_stride,
                            int64_t num_slots, int32_t elem_bytes, void* stream);
 
 /*
+ * 4-bit KV cache.  One layer's keys (and values) are uint8
+ * [num_blocks, Hkv, block_size, 80], contiguous and 16-byte aligned: one
+ * record of 80 bytes per (token, kv head), records of consecutive tokens of a
+ * head next to each other; slot = block * block_size + token, as in the
+ * 16-bit cache.  A record is 64 bytes of codes (16 per group of 32 head
+ * dimensions) and, per group, one 32-bit word: scale s in the low half,
+ * minimum m in the high half, both in `dtype` (bf16 or fp16).  A word of codes
+ * holds dimensions 8w .. 8w + 7: nibbles 0-3 the even ones, 4-7 the odd ones.
+ *     m = min x, s = (max x - m) / 15 in fp32 rounded to dtype (0 if < 2^-100),
+ *     code = min(15, rint((x - m) / s)), value = s * code + m;
+ * a group whose max - min is not finite gets s = m = NaN, codes 0.  A cache is
+ * read with the dtype it was written with.  head_dim is 128.
+ *
+ * store: quantises key / value rows [num_tokens, Hkv, 128] into the records of
+ * slot_mapping[t]; slots of -1 or outside the cache are skipped, the others
+ * must be unique within one call.
+ * load: the reverse, rows of `dtype`; slots of -1 or outside the cache give
+ * zeros.
+ * gather: rows cu_seqlens[i] + p = token p of sequence i, through
+ * block_tables (rows of block_table_width entries, block_table_stride apart;
+ * stride 0 shares one row); rows before cu_seqlens[0], from
+ * cu_seqlens[num_seqs] on or past total_tokens are not written; tokens of a
+ * block id outside the cache or past the table give zeros.
+ * All are bound by memory and launch one kernel; any 2-byte aligned rows are
+ * taken, 16-byte aligned ones by vector accesses.
+ */
+B200_API int32_t b200_store_kvcache_q4(const void* key, int64_t key_stride,
+                              const void* value, int64_t value_stride,
+                              void* k_cache, void* v_cache,
+                              const int32_t* slot_mapping, int32_t num_tokens,
+                              int32_t num_kv_heads, int32_t head_dim,
+                              int32_t num_blocks, int32_t block_size,
+                              int32_t dtype, void* stream);
+
+B200_API int32_t b200_load_kvcache_q4(void* key, int64_t key_stride,
+                             void* value, int64_t value_stride,
+                             const void* k_cache, const void* v_cache,
+                             const int32_t* slot_mapping, int32_t num_tokens,
+                             int32_t num_kv_heads, int32_t head_dim,
+                             int32_t num_blocks, int32_t block_size,
+                             int32_t dtype, void* stream);
+
+B200_API int32_t b200_gather_kvcache_q4(void* key, int64_t key_stride,
+                               void* value, int64_t value_stride,
+                               const void* k_cache, const void* v_cache,
+                               const int32_t* cu_seqlens,
+                               const int32_t* block_tables, int64_t block_table_stride,
+                               int32_t block_table_width, int32_t num_seqs,
+                               int32_t total_tokens, int32_t num_kv_heads, int32_t head_dim,
+                               int32_t num_blocks, int32_t block_size,
+                               int32_t dtype, void* stream);
+
+/*
+ * b200_paged_attention over a 4-bit cache: same queries, limits
+ * (query_len * Hq/Hkv <= 16, batch <= 2048, block_size a multiple of 128),
+ * masks, padding rows and workspace (b200_paged_attention_workspace_size,
+ * b200_workspace_error).  Block tables are rows of block_table_width entries,
+ * block_table_stride apart; a tile of a block id outside the cache counts as
+ * tokens of zeros.  Scores, softmax statistics and sums are fp32; p * s is
+ * rounded to fp16 for the product with the codes.  Queries and stored scales
+ * are expected between 2^-60 and 2^60 in magnitude.
+ */
+B200_API int32_t b200_paged_attention_q4(void* out, const void* q, int64_t q_stride_token,
+                                const void* k_cache, const void* v_cache,
+                                int32_t num_blocks, int32_t block_size,
+                                const int32_t* block_tables, int64_t block_table_stride,
+                                int32_t block_table_width, const int32_t* context_lens,
+                                int32_t batch, int32_t query_len,
+                                int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                float softmax_scale, int32_t dtype,
+                                void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Fused q/k RMSNorm + rotary embedding + KV-cache scatter for Qwen3 layers.
  * Replaces, in one pass over the fused QKV projection output `qkv`
  * ([num_tokens, (Hq + 2 Hkv) * D], token stride qkv_stride):

@@ -1,0 +1,121 @@
+// Records of the 4-bit KV cache, shared by the kernels that write and read them.
+//
+// One record of 80 bytes stands for the 128 values of one (token, kv head):
+//   bytes  0-63  codes, 16 bytes for each of the four groups of 32 head dimensions;
+//   bytes 64-79  one 32-bit word per group: scale s (low half) and minimum m (high half)
+//                in the model's 16-bit type.
+// A value is s * code + m.  A 32-bit word of codes holds eight consecutive dimensions, the
+// even ones in its low half and the odd ones in its high half (nibble i of a half is dimension
+// 2 i, 2 i + 1): masking a word, shifted by 4 i, with 0x000f000f leaves the codes of two
+// neighbouring dimensions in the two halves of a register, where a 16-bit matrix operand
+// wants them.  Records of consecutive tokens of one head are contiguous
+// ([num_blocks][num_kv_heads][block_size][80]), so that a tile of a head's tokens is one bulk
+// copy; the 80-byte stride puts eight records' 16-byte rows into eight different bank groups.
+#pragma once
+
+#include <cfloat>
+
+#include "common.cuh"
+
+namespace b200 {
+namespace q4 {
+
+constexpr int kD = 128;
+constexpr int kGroups = 4;          // groups of 32 dimensions
+constexpr int kRecord = 80;         // bytes
+constexpr int kParams = 64;         // byte offset of the scales and minima
+constexpr float kMinScale = 7.888609052210118e-31f;  // 2^-100: smaller scales are stored as 0
+
+template <bool BF16>
+__device__ __forceinline__ float lo_f(uint32_t w) {
+    if constexpr (BF16) return __uint_as_float(w << 16);
+    else return __half2float(__ushort_as_half(uint16_t(w)));
+}
+template <bool BF16>
+__device__ __forceinline__ float hi_f(uint32_t w) {
+    if constexpr (BF16) return __uint_as_float(w & 0xffff0000u);
+    else return __half2float(__ushort_as_half(uint16_t(w >> 16)));
+}
+
+// Minimum / maximum of packed pairs; a NaN in either operand gives NaN.
+template <bool BF16>
+__device__ __forceinline__ uint32_t min2_nan(uint32_t a, uint32_t b) {
+    uint32_t d;
+    if constexpr (BF16) asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    else asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b) {
+    uint32_t d;
+    if constexpr (BF16) asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    else asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+
+// Quantises eight consecutive dimensions per lane (x: four packed pairs); the four lanes of an
+// aligned quad hold one group.  Returns the lane's word of codes and the group's parameter word.
+//
+//   m = min x, s = (max x - m) / 15 rounded to the model's type (0 below 2^-100),
+//   code = min(15, rint((x - m) / s)), ties to even; a group whose max - min is not finite
+//   gets s = m = NaN and codes 0.
+// The codes are those of a correctly rounded quotient: with y = 1/s correctly rounded and q0
+// the rounded product (x - m) y, q = q0 + ((x - m) - q0 s) y in two fused operations is the
+// correctly rounded quotient (Markstein 1990; s has at most 11 significant bits and at least
+// 2^-100, so no step under- or overflows), two instructions per pair instead of a division.
+template <bool BF16>
+__device__ __forceinline__ uint32_t quantise8(const uint32_t (&x)[4], uint32_t& params) {
+    const uint32_t mn = min2_nan<BF16>(min2_nan<BF16>(x[0], x[1]), min2_nan<BF16>(x[2], x[3]));
+    const uint32_t mx = max2_nan<BF16>(max2_nan<BF16>(x[0], x[1]), max2_nan<BF16>(x[2], x[3])) ^ 0x80008000u;
+    // {min, -max} of the lane, then of the quad: one minimum serves both.
+    uint32_t r = min2_nan<BF16>(__byte_perm(mn, mx, 0x5410), __byte_perm(mn, mx, 0x7632));
+    r = min2_nan<BF16>(r, __shfl_xor_sync(0xffffffffu, r, 1));
+    r = min2_nan<BF16>(r, __shfl_xor_sync(0xffffffffu, r, 2));
+    const float lo = lo_f<BF16>(r), span = -hi_f<BF16>(r) - lo;
+    const bool finite = span <= FLT_MAX;
+    uint32_t sbits = to_bits16<BF16>(__fdiv_rn(span, 15.f));
+    float s = lo_f<BF16>(sbits);
+    if (s < kMinScale) {
+        s = 0.f;
+        sbits = 0;
+    }
+    const float inv = s > 0.f ? __frcp_rn(s) : 0.f;
+    params = finite ? (sbits | (r << 16)) : 0x7fff7fffu;  // the all-ones pattern is NaN in both types
+    uint32_t even = 0, odd = 0;
+#pragma unroll
+    for (int i = 3; i >= 0; --i) {
+        const float2 d = fsub2(make_float2(lo_f<BF16>(x[i]), hi_f<BF16>(x[i])), make_float2(lo, lo));
+        const float2 q0 = fmul2(d, make_float2(inv, inv));
+        const float2 e = ffma2(q0, make_float2(-s, -s), d);
+        float2 q = ffma2(e, make_float2(inv, inv), q0);
+        q.x = fminf(q.x, 15.f);
+        q.y = fminf(q.y, 15.f);
+        // rint by the magic constant 1.5 * 2^23: the code lands in the low mantissa bits.  Shifting
+        // moves the constant's own bits (22 and up) past bit 15, which is all that is kept.
+        const float2 t = fadd2(q, make_float2(12582912.f, 12582912.f));
+        even = even * 16 + __float_as_uint(t.x);
+        odd = odd * 16 + __float_as_uint(t.y);
+    }
+    const uint32_t word = __byte_perm(even, odd, 0x5410);
+    return finite ? word : 0u;
+}
+
+// The eight values of a word of codes, rounded to the model's type (four packed pairs).
+template <bool BF16>
+__device__ __forceinline__ uint4 dequantise8(uint32_t word, uint32_t params) {
+    const float s = lo_f<BF16>(params), m = hi_f<BF16>(params);
+    uint32_t y[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        // 2^23 + code is exact in fp32, and so is s * code: one rounding in the sum, one to 16 bits.
+        const float2 c = fsub2(make_float2(__uint_as_float(0x4b000000u | ((word >> (4 * i)) & 15u)),
+                                           __uint_as_float(0x4b000000u | ((word >> (16 + 4 * i)) & 15u))),
+                               make_float2(8388608.f, 8388608.f));
+        const float2 v = ffma2(c, make_float2(s, s), make_float2(m, m));
+        y[i] = pack2<BF16>(v.x, v.y);
+    }
+    return make_uint4(y[0], y[1], y[2], y[3]);
+}
+
+}  // namespace q4
+}  // namespace b200
