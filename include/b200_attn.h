@@ -139,13 +139,17 @@ B200_API int32_t b200_gather_kvcache_q4(void* key, int64_t key_stride,
 /*
  * b200_paged_attention over a 4-bit cache: same queries, limits
  * (query_len * Hq/Hkv <= 16, batch <= 2048, block_size a multiple of 128),
- * masks, padding rows and workspace (b200_paged_attention_workspace_size,
- * b200_workspace_error).  Block tables are rows of block_table_width entries,
+ * masks and padding rows.  The workspace works as there
+ * (b200_paged_attention_q4_workspace_size bytes for the current device,
+ * 256-byte aligned, zero-filled once, whatever the batch; a call leaves its
+ * counters zeroed; b200_workspace_error reads its error word).  Block tables are rows of block_table_width entries,
  * block_table_stride apart; a tile of a block id outside the cache counts as
  * tokens of zeros.  Scores, softmax statistics and sums are fp32; p * s is
  * rounded to fp16 for the product with the codes.  Queries and stored scales
  * are expected between 2^-60 and 2^60 in magnitude.
  */
+B200_API size_t b200_paged_attention_q4_workspace_size(int32_t query_len, int32_t group_size);
+
 B200_API int32_t b200_paged_attention_q4(void* out, const void* q, int64_t q_stride_token,
                                 const void* k_cache, const void* v_cache,
                                 int32_t num_blocks, int32_t block_size,

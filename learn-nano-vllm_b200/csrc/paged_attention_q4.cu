@@ -1,79 +1,146 @@
 // Paged multi-query attention for decode and speculative verification over a 4-bit KV cache:
 // the call of nanovllm/layers/attention.py:71-74 on records of kv_q4.cuh.
 //
-// Work decomposition, scheduling, split-K merge and the bounded waits are those of
-// paged_attention.cu (paged_plan.cuh); a stage is 128 records of keys and 128 of values, two
-// contiguous 10 KiB bulk copies.
-//
 // Mathematics.  A cached value is s n + m with n the 4-bit code and one (s, m) per group of 32
 // head dimensions, so per query row and token
-//     q . k = sum_g ( s_g (q_g . n_g) + m_g sum(q_g) ),      o_g = sum_t (p_t s_tg) n_tg + sum_t p_t m_tg.
+//     q . k = sum_g s_g (q_g . n_g) + sum_g m_g sum(q_g),    o_g = sum_t (p_t s_tg) n_tg + sum_t p_t m_tg.
 // The codes themselves are the matrix operands: a nibble in the low bits of an fp16 lane is the
 // subnormal n * 2^-24 (16 n * 2^-24 one nibble up), exactly, so that a mask turns a word of
 // codes into operands of mma.sync.m16n8k16 and nothing is converted.  The powers of two are
-// undone in fp32; the queries that meet the second nibble carry a factor 1/16.  Scales and
-// minima are applied in fp32 on the results (keys) and on the probabilities (values); p s is
-// rounded to fp16 (2^-12 relative), q is exact in fp16 after scaling each row by a power of two.
-//
-// As in the 16-bit kernel's transposed form tokens are the M of the matrix products and query
-// rows their N (8 per tile, NT tiles): S^T = K Q^T, O^T += V^T (P s)^T.  ldmatrix hands lane
-// (g, c) word c of token g's four groups; its transposed form hands it half-word g of tokens
-// 2 c and 2 c + 1, again one nibble per token in either half of a register.
+// undone in fp32; the queries that meet a second nibble carry a factor 1/16.
+//   * Tokens are the M of both products' operands: S^T = K Q^T and O^T = V^T (P s)^T, query rows
+//     their N of 8.  ldmatrix hands lane (g, c) word c of token g's four groups, the transposed form
+//     half-word g of tokens 2 c and 2 c + 1: one nibble per dimension (token) in either half of a
+//     register both times.  For the values the second operand row is the byte n + 16 n' as it is:
+//     n' comes out by subtraction at the end, which saves a mask.  P^T turns into a B operand by
+//     movmatrix.
+//   * The words (s, m) of a token are an operand as they are: against the rows (0, sum(q_g)) they
+//     give the minima's part of the score; against P^T, transposed, sum_t p m, and a row of ones
+//     beside them the softmax sum.  sum(q_g) and p enter as two 16-bit parts (hi + lo).
+//   * The scales are applied in fp32, to the products with the key codes and to the probabilities;
+//     p s is rounded to fp16 for the product with the value codes (2^-12; two parts for fp16
+//     models, whose outputs would show it).
 //
 // Ranges.  A row's probabilities are 2^(x - r) with r = (lazy running maximum) + E, where 2^E
 // follows the largest value scale the warp has met (raised when a scale exceeds 2^7 times it):
-// p s then stays below 2^15 and small scales do not underflow fp16.
+// p s then stays below 2^15 and small scales do not underflow fp16.  Queries are scaled by a
+// power of two per row (largest element in [8, 16)), exactly but for elements below 2^-18 of it.
+//
+// Work split.  The tiles of 128 tokens of all (sequence, kv head) pairs in a row, sequence by
+// sequence, are cut into equal runs, one per CTA, all CTAs resident: no claims, no tail, a
+// sequence is split only where a run ends, and a long one over as many CTAs as its share of the
+// work.  Every CTA plans its run from context_lens (no host sync: the call can be captured).
+// A CTA leaves at most two partial results, its first and its last; the warp that finishes the
+// last chunk of a split pair (one counter per consumer warp) merges its share of the outputs.
+//
+// CTA.  Four consumer warps and a producer warp, three CTAs per SM (15 warps leave 128 registers
+// a thread).  A stage is 128 records of keys and 128 of values, two contiguous 10 KiB bulk copies
+// into a ring of three, guarded by full / empty mbarriers.  Up to 8 query rows each consumer warp
+// takes 32 of a tile's tokens; for 9 to 16 rows two warps take rows 0-7 and two rows 8-15, 64
+// tokens each.  The warps keep their own softmax states and combine them through shared memory at the
+// end of an item.  Every wait is bounded (kWaitLimitNs, or the test limit).
 #include <cfloat>
 #include <climits>
+#include <type_traits>
 
 #include "kv_q4.cuh"
-#include "paged_plan.cuh"
 
 namespace b200 {
-namespace pa {
+namespace pq4 {
 namespace {
 
 using q4::hi_f;
+using q4::kD;
 using q4::kGroups;
 using q4::kRecord;
 using q4::lo_f;
 
+constexpr int kTile = 128;  // tokens per stage
+constexpr int kWarps = 4;   // consumer warps
+constexpr int kConsumers = kWarps * 32;
+constexpr int kThreads = kConsumers + 32;
+constexpr int kCtas = 3;    // per SM
+constexpr int kStages = 3;
+constexpr int kQBufs = 2;
 constexpr int kKvBytes = kTile * kRecord;  // keys (or values) of one stage
-constexpr int kStage = 2 * kKvBytes;
-constexpr int32_t kNoPage = 4;             // header flag: the tile's block id is not in the cache
-constexpr float kNone = -1e30f;            // reference of a row that has met no token
-constexpr int kExpMin = -60, kExpMax = 60; // bounds of E and of the query rows' exponents
+constexpr int kStageBytes = 2 * kKvBytes;
+constexpr int kMaxBatch = 2048;
+constexpr int kPairCost = 2;  // what a (sequence, kv head) pair costs beside its tiles, in tiles
+constexpr float kLazyMax = 8.f;  // log2 headroom before a row's running maximum is raised
+constexpr float kNone = -1e30f;  // reference of a row that has met no token
+constexpr int kExpMax = 60;      // bound of |E| and of the query rows' exponents
+// Least E.  fp16 operands hold p * 2^-E itself: below 2^15 with p <= 2^kLazyMax.
+template <bool BF16>
+constexpr int kExpMin = BF16 ? -kExpMax : -7;
 
-struct Q4Params {
-    Params base;
+// All CTAs of the grid are resident (three per SM).
+int grid_ctas() { return device_sm_count() * kCtas; }
+
+// Workspace: control words ([2] error word), counters of the CTAs' last items (one per consumer
+// warp), two partial results per CTA and, once per consumer warp, their log-sum-exps.
+constexpr size_t kCtrlBytes = 256;
+size_t fixed_bytes(int ctas) { return kCtrlBytes + ((size_t(ctas) * kWarps * 4 + 255) & ~size_t(255)); }
+size_t workspace_bytes(int rows, int ctas) {
+    return (fixed_bytes(ctas) + size_t(2) * ctas * rows * (kD + kWarps) * 4 + 255) & ~size_t(255);
+}
+
+struct Params {
+    const uint16_t* q;
+    int64_t q_stride;
+    uint16_t* out;
     const uint8_t* k;
     const uint8_t* v;
+    const int32_t* block_tables;
+    int64_t bt_stride;
+    int32_t bt_width;
+    const int32_t* context_lens;
+    int32_t batch, lq, hq, hkv, group, rows, block_size, num_blocks;
+    int32_t group_inv;  // ceil(2^16 / group): r / group = (r * group_inv) >> 16 for r < 16
+    float scale_log2;
+    uint64_t wait_ns;       // limit of every wait (kWaitLimitNs; shorter under the idle-producer test)
+    int32_t idle_producer;  // test hook: the producer issues nothing, so the consumers' first wait runs out
+    int32_t* error;
+    int32_t* counters;
+    float* part_o;    // [2 * CTAs][rows][kD]
+    float* part_lse;  // [2 * CTAs][kWarps][rows]
 };
 
-template <int NT>
+// What a tile's warps need, and what is only needed at the end of an item.
+struct Header {
+    int32_t tile, flags, ctx, b;
+    int32_t h, first, nch, pad;  // CTA of the pair's first chunk, number of chunks
+};
+enum : int32_t { kFirst = 1, kLast = 2, kNoPage = 4, kQBuf = 8 };
+
+// ROWS16: 9 to 16 query rows.
+template <bool ROWS16>
 struct Cfg {
-    // Up to 8 query rows: two CTAs per SM, one of them computes while the other waits or combines.
-    static constexpr int kCtas = NT == 1 ? 2 : 1;
-    static constexpr int kStages = NT == 1 ? 4 : 7;
+    static constexpr int kHalves = ROWS16 ? 2 : 1;              // groups of 8 query rows
+    static constexpr int kSlices = kWarps / kHalves;            // warps that share a group of rows
+    static constexpr int kWarpTokens = kTile / kSlices;
+    static constexpr int kPassRows = 4 / kHalves;               // rows of a group combined at a time
 };
 
-template <int NT>
+constexpr int kRowPad = kD + 1;  // floats: the lanes of a fragment write 32 different banks
+
+template <bool ROWS16>
 struct Smem {
-    alignas(128) uint8_t stages[Cfg<NT>::kStages][kStage];
-    uint8_t qbuf[Cfg<NT>::kStages][8 * NT * kD * 2];
-    float co[kConsumerWarps / 2][8 * NT][kD];
-    float cm[kConsumerWarps][8 * NT];
-    float cl[kConsumerWarps][8 * NT];
-    Header hdr[Cfg<NT>::kStages];
-    uint64_t full[Cfg<NT>::kStages];
-    uint64_t empty[Cfg<NT>::kStages];
+    alignas(128) uint8_t stages[kStages][kStageBytes];
+    uint8_t qbuf[kQBufs][8 * Cfg<ROWS16>::kHalves * kD * 2];
+    float co[kWarps][Cfg<ROWS16>::kPassRows][kRowPad];
+    float cm[kWarps][Cfg<ROWS16>::kPassRows];
+    float cl[kWarps][Cfg<ROWS16>::kPassRows];
+    alignas(16) uint32_t ones[4];  // a row of ones in the model's type
+    Header hdr[kStages];
+    uint64_t full[kStages];
+    uint64_t empty[kStages];
     uint64_t cbar;
-    int32_t off[kMaxBatch + 1];
-    int32_t red[kThreads / 32 + 1];
-    int32_t flag;
+    int32_t off[kConsumers];  // length before each entry of ceil(batch / 128) sequences
+    int32_t red[kWarps];
     int32_t err;
 };
-static_assert(sizeof(Smem<1>) <= 233472 / 2 - 1024 && sizeof(Smem<2>) <= 232448, "shared memory over the SM's");
+static_assert(sizeof(Smem<false>) <= 233472 / kCtas - 1024 && sizeof(Smem<true>) <= 233472 / kCtas - 1024,
+              "shared memory over the SM's");
 
 __device__ __forceinline__ void bulk_load_hint(void* dst, const void* src, uint32_t bytes, uint64_t* bar,
                                                uint64_t policy) {
@@ -84,571 +151,730 @@ __device__ __forceinline__ void bulk_load_hint(void* dst, const void* src, uint3
         : "memory");
 }
 
+// D(16x8, f32) = A(16x16) * B(16x8) + C.  Not volatile, unlike common.cuh's: the compiler may order
+// these among the loads and conversions.
+template <bool BF16>
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (BF16) {
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    } else {
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+}
+// The same with C = 0, which takes no registers.
+template <bool BF16>
+__device__ __forceinline__ void mma_zero(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (BF16) {
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+    } else {
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+    }
+}
+// movmatrix_t (common.cuh), not volatile.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
 __device__ __forceinline__ float exp2_int(int e) { return __int_as_float((127 + e) << 23); }  // -126 <= e <= 127
 
-template <bool BF16, int NT>
-__global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_kernel(const __grid_constant__ Q4Params qp) {
-    constexpr int NS = Cfg<NT>::kStages;
-    const Params& p = qp.base;
+// Two 16-bit parts of a pair of floats: hi + lo = x to 16 (bf16) or 22 (fp16) bits.
+template <bool BF16>
+__device__ __forceinline__ void split2(float2 x, uint32_t& hi, uint32_t& lo) {
+    if constexpr (BF16) hi = __byte_perm(__float_as_uint(x.x), __float_as_uint(x.y), 0x7632);  // truncated
+    else hi = pack2<false>(x.x, x.y);
+    const float2 r = fsub2(x, make_float2(lo_f<BF16>(hi), hi_f<BF16>(hi)));
+    lo = pack2<BF16>(r.x, r.y);
+}
+
+// A pair of 16-bit floats with its infinities and NaNs replaced by zeros.
+template <bool BF16>
+__device__ __forceinline__ uint32_t finite2(uint32_t w) {
+    constexpr uint32_t kExp = BF16 ? 0x7f80u : 0x7c00u;
+    if ((w & kExp) == kExp) w &= 0xffff0000u;
+    if (((w >> 16) & kExp) == kExp) w &= 0xffffu;
+    return w;
+}
+
+// Barrier of the consumer threads, bounded.  False, for the whole warp alike, when a lane's wait ran out.
+__device__ __forceinline__ bool consumer_wait(uint64_t* bar, uint32_t& phase, uint64_t limit_ns) {
+    const bool ok = mbar_wait_spin(bar, phase, limit_ns);
+    phase ^= 1;
+    return __all_sync(0xffffffffu, ok);
+}
+
+__device__ __forceinline__ int tiles_of(int ctx, int cap) { return (min(max(ctx, 0), cap) + kTile - 1) / kTile; }
+
+// Length of a pair of nt tiles on the line that is cut into runs: its tiles, then kPairCost.
+__device__ __forceinline__ int span_of(int nt) { return nt > 0 ? nt + kPairCost : 0; }
+
+// Offset of output row r (query r / group, head r % group of kv head h) of sequence b.
+__device__ __forceinline__ int64_t out_row(const Params& p, int b, int h, int r) {
+    const int j = (r * p.group_inv) >> 16;
+    return ((int64_t(b) * p.lq + j) * p.hq + h * p.group + (r - j * p.group)) * kD;
+}
+
+// Merges the chunks of a split pair for the rows [row0, row0 + n) and this warp's share of each pass
+// of kPassRows of them; called by the warp that finished the last chunk.
+template <bool BF16, bool ROWS16>
+__device__ __forceinline__ void merge_share(const Params& p, const Header& hd, int row0, int n, int warp, int lane) {
+    using C = Cfg<ROWS16>;
+    for (int r0 = 0; r0 < n; r0 += C::kPassRows) {
+        const int share = min(C::kPassRows, n - r0) * (kD / C::kSlices);
+        for (int i = 4 * lane; i < share; i += 128) {
+            const int e = (row0 + r0) * kD + (warp % C::kSlices) * share + i, r = e >> 7, d = e & (kD - 1);
+            float m = -INFINITY, den = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+            constexpr int kFlight = 8;  // chunks whose loads are in flight
+            for (int c0 = 0; c0 < hd.nch; c0 += kFlight) {
+                float lse[kFlight];
+                float4 x[kFlight];
+                float mx = m;
+#pragma unroll
+                for (int u = 0; u < kFlight; ++u) {
+                    lse[u] = -INFINITY;
+                    x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (c0 + u < hd.nch) {
+                        const int64_t slot = 2 * int64_t(hd.first + c0 + u) + (c0 + u == 0 ? 1 : 0);
+                        lse[u] = __ldcg(p.part_lse + (slot * kWarps + warp) * p.rows + r);
+                        x[u] = __ldcg(reinterpret_cast<const float4*>(p.part_o + (slot * p.rows + r) * kD + d));
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < kFlight; ++u) mx = fmaxf(mx, lse[u]);
+                if (mx == -INFINITY) continue;
+                const float sc = fast_exp2(m - mx);
+                den *= sc;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) acc[k] *= sc;
+#pragma unroll
+                for (int u = 0; u < kFlight; ++u) {
+                    const float w = lse[u] == -INFINITY ? 0.f : fast_exp2(lse[u] - mx);
+                    den += w;
+                    acc[0] = fmaf(w, x[u].x, acc[0]);
+                    acc[1] = fmaf(w, x[u].y, acc[1]);
+                    acc[2] = fmaf(w, x[u].z, acc[2]);
+                    acc[3] = fmaf(w, x[u].w, acc[3]);
+                }
+                m = mx;
+            }
+            const float inv = den == 0.f ? 0.f : __fdividef(1.f, den);
+            *reinterpret_cast<uint2*>(p.out + out_row(p, hd.b, hd.h, r) + d) =
+                make_uint2(pack2<BF16>(acc[0] * inv, acc[1] * inv), pack2<BF16>(acc[2] * inv, acc[3] * inv));
+        }
+    }
+}
+
+template <bool BF16, bool ROWS16>
+__global__ void __launch_bounds__(kThreads, kCtas) paged_attention_q4_kernel(const __grid_constant__ Params p) {
+    using C = Cfg<ROWS16>;
     extern __shared__ uint8_t smem_raw[];
-    Smem<NT>& sm = *reinterpret_cast<Smem<NT>*>(smem_raw);
+    Smem<ROWS16>& sm = *reinterpret_cast<Smem<ROWS16>*>(smem_raw);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int cap = p.bt_width * p.block_size;  // tokens addressable through the block table
 
     if (tid == 0) {
-        for (int s = 0; s < NS; ++s) {
+        for (int s = 0; s < kStages; ++s) {
             mbar_init(&sm.full[s], 1);
-            mbar_init(&sm.empty[s], kConsumerWarps);
+            mbar_init(&sm.empty[s], kWarps);
         }
         mbar_init(&sm.cbar, kConsumers);
         sm.err = 0;
+        for (int i = 0; i < 4; ++i) sm.ones[i] = BF16 ? 0x3f803f80u : 0x3c003c00u;
         fence_mbar_init();
     }
-    // The producer's first claim does not depend on the plan: its latency overlaps the planning.
-    const bool producer = warp == kConsumerWarps && lane == 0 && !p.idle_producer;
-    const int first_claim = producer ? atomicAdd(&p.ctrl[0], 1) : 0;
-    const Plan pl = plan_items(p, sm.off, sm.red);
 
-    // Rows without a cached token (CUDA-graph padding) have no items and get a zero output.
+    // ---- plan: this CTA's run ------------------------------------------
+    const int run = (p.batch + kConsumers - 1) / kConsumers;  // sequences per entry of off[]
+    int total;                                                // length of all pairs
+    {
+        int mine = 0, before = 0;
+        if (warp < kWarps) {
+            for (int b = tid * run; b < min((tid + 1) * run, p.batch); ++b) mine += span_of(tiles_of(p.context_lens[b], cap));
+            before = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, before, o);
+                if (lane >= o) before += y;
+            }
+            if (lane == 31) sm.red[warp] = before;
+        }
+        __syncthreads();
+        total = 0;
+        for (int w = 0; w < kWarps; ++w) {
+            if (w < warp) before += sm.red[w];
+            total += sm.red[w];
+        }
+        if (warp < kWarps) sm.off[tid] = before - mine;
+        total *= p.hkv;
+        __syncthreads();
+    }
+    const int quota = max(1, (total + int(gridDim.x) - 1) / int(gridDim.x));
+    const int begin = int(min(int64_t(blockIdx.x) * quota, int64_t(total))), end = min(begin + quota, total);
+
+    // Rows without a cached token (CUDA-graph padding) have no tiles and get a zero output.
     const int64_t row_vec = int64_t(p.lq) * p.hq * kD / 8;  // uint4 per batch row
     for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
-        if (sm.off[b + 1] == sm.off[b]) {
+        if (p.context_lens[b] <= 0) {
             uint4* o = reinterpret_cast<uint4*>(p.out) + b * row_vec;
             for (int64_t i = tid; i < row_vec; i += kThreads) o[i] = make_uint4(0, 0, 0, 0);
         }
     }
+    if (begin >= end) return;
 
-    if (warp == kConsumerWarps) {
+    if (warp == kWarps) {
         // ------------------------------------------------------------ producer
-        if (producer) {
+        if (lane == 0 && !p.idle_producer) {
             const uint64_t pol = l2_policy_evict_first();
             const uint32_t q_bytes = uint32_t(p.group) * kD * 2;  // one query token's rows of this kv head
-            int stage = 0;
+            // First pair of the run: its entry of off[] by binary search, then along the entry.
+            int lo = 0, hi = kConsumers;
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (sm.off[mid] * p.hkv <= begin) lo = mid; else hi = mid;
+            }
+            int b = lo * run, at = sm.off[lo] * p.hkv;  // `at`: where the current pair begins
+            int ctx = min(p.context_lens[b], cap), nt = tiles_of(ctx, cap);
+            while (at + span_of(nt) * p.hkv <= begin) {
+                at += span_of(nt) * p.hkv;
+                ctx = min(p.context_lens[++b], cap);
+                nt = tiles_of(ctx, cap);
+            }
+            int h = (begin - at) / span_of(nt);
+            at += h * span_of(nt);
+            int t = begin - at;
+            // The next sequence's length and the next tile's page are loaded one step ahead.
+            int ctx_next = p.context_lens[min(b + 1, p.batch - 1)];
+            auto page_of = [&](int seq, int tile) { return p.block_tables[seq * p.bt_stride + (tile * kTile) / p.block_size]; };
+            // The first tile of the next pair that has one, if it lies in this run.
+            auto next_pair = [&](int& b, int& h, int& t, int& nt, int& ctx, int& at) {
+                t = 0;
+                at += span_of(nt);
+                if (at >= end || ++h < p.hkv) return;
+                h = 0;
+                do {
+                    ++b;
+                    ctx = min(ctx_next, cap);
+                    nt = tiles_of(ctx, cap);
+                    ctx_next = p.context_lens[min(b + 1, p.batch - 1)];
+                } while (nt == 0);
+            };
+            if (t >= nt) next_pair(b, h, t, nt, ctx, at);
+            int blk = at + t < end ? page_of(b, t) : 0;
+
+            int stage = 0, qb = 0;
             uint32_t phase = 0;
-            int64_t fills = 0;
+            int fills = 0;
+            int q_fill[kQBufs] = {-kStages, -kStages};  // fill that brought the query rows of each buffer
             bool ok = true;
-            ItemMeta cur, nxt;
-            cur.item = pl.total_items;
-            if (first_claim < pl.total_items) fetch_meta(cur, first_claim, p, sm.off, pl.total_full, pl.chunk, pl.cap);
-            while (ok && cur.item < pl.total_items) {
-                const int ctx = min(cur.ctx, pl.cap);
-                const int nt = (ctx + kTile - 1) / kTile;
-                const int t0 = cur.t0;
-                const int t1 = int(min(int64_t(nt), t0 + pl.chunk));
-                const int32_t* bt = p.block_tables + int64_t(cur.b) * p.bt_stride;
-                const int t_claim = max(t0, t1 - kClaimAhead);
-                nxt.item = pl.total_items;
-                for (int t = t0; t < t1; ++t) {
-                    if (!mbar_wait(&sm.empty[stage], phase ^ 1, p.wait_ns)) {
-                        atomicOr(&p.ctrl[2], DEV_ERR_WAIT_EMPTY);
+            int first_flag = kFirst;
+            while (at + t < end) {
+                // Where the walk goes next.
+                int b2 = b, h2 = h, t2 = t + 1, nt2 = nt, ctx2 = ctx, at2 = at;
+                if (t2 == nt) next_pair(b2, h2, t2, nt2, ctx2, at2);
+                const bool more = at2 + t2 < end, last = at2 != at || !more;
+                const int blk2 = more ? page_of(b2, t2) : 0;
+                if (!mbar_wait(&sm.empty[stage], phase ^ 1, p.wait_ns)) {
+                    ok = false;
+                    break;
+                }
+                if (first_flag) {
+                    // The query buffer's last rows were taken with their item's first tile.
+                    const int f = q_fill[qb];
+                    if (f > fills - kStages && f >= 0 && !mbar_wait(&sm.empty[f % kStages], (f / kStages) & 1, p.wait_ns)) {
                         ok = false;
                         break;
                     }
-                    const bool first = t == t0;
-                    const int pos = t * kTile;
-                    const int lb = pos / p.block_size;
-                    int blk;
-                    const int j = lb - cur.page0;
-                    if (j < kPrefetchPages) {
-                        blk = cur.blk[0];
-#pragma unroll
-                        for (int u = 1; u < kPrefetchPages; ++u)
-                            if (j == u) blk = cur.blk[u];
-                    } else {
-                        blk = bt[lb];
-                    }
-                    const bool page = blk >= 0 && blk < p.num_blocks;
-                    Header& hd = sm.hdr[stage];
-                    hd.item = cur.item;
-                    hd.b = cur.b;
-                    hd.h = cur.h;
-                    hd.tile = t;
-                    hd.flags = (first ? kFirst : 0) | (t == t1 - 1 ? kLast : 0) | (page ? 0 : kNoPage);
-                    hd.ctx = ctx;
-                    hd.nchunks = cur.nchunks;
-                    hd.slot0 = cur.slot0;
-                    mbar_arrive_expect_tx(&sm.full[stage], (page ? uint32_t(kStage) : 0u) + (first ? q_bytes * p.lq : 0u));
-                    uint8_t* st = sm.stages[stage];
-                    if (page) {
-                        const int64_t o = ((int64_t(blk) * p.hkv + cur.h) * p.block_size + (pos - lb * p.block_size)) * kRecord;
-                        bulk_load_hint(st, qp.k + o, kKvBytes, &sm.full[stage], pol);
-                        bulk_load_hint(st + kKvBytes, qp.v + o, kKvBytes, &sm.full[stage], pol);
-                    }
-                    if (first) {
-                        const uint16_t* qsrc = p.q + int64_t(cur.b) * p.lq * p.q_stride + int64_t(cur.h) * p.group * kD;
-                        for (int jq = 0; jq < p.lq; ++jq)
-                            bulk_load(sm.qbuf[stage] + jq * q_bytes, qsrc + int64_t(jq) * p.q_stride, q_bytes,
-                                      &sm.full[stage]);
-                    }
-                    ++fills;
-                    if (++stage == NS) { stage = 0; phase ^= 1; }
-                    if (t == t_claim) {  // the claim's dependent loads overlap the tiles in flight
-                        const int claim = atomicAdd(&p.ctrl[0], 1);
-                        if (claim < pl.total_items) fetch_meta(nxt, claim, p, sm.off, pl.total_full, pl.chunk, pl.cap);
-                    }
+                    q_fill[qb] = fills;
                 }
-                cur = nxt;
+                const bool page = blk >= 0 && blk < p.num_blocks;
+                Header& hd = sm.hdr[stage];
+                hd.tile = t;
+                hd.flags = first_flag | (last ? kLast : 0) | (page ? 0 : kNoPage) | (qb ? kQBuf : 0);
+                hd.ctx = ctx;
+                hd.b = b;
+                hd.h = h;
+                hd.first = at / quota;
+                hd.nch = (at + nt - 1) / quota - hd.first + 1;
+                mbar_arrive_expect_tx(&sm.full[stage],
+                                      (page ? uint32_t(kStageBytes) : 0u) + (first_flag ? q_bytes * p.lq : 0u));
+                uint8_t* st = sm.stages[stage];
+                if (page) {
+                    const int64_t o = ((int64_t(blk) * p.hkv + h) * p.block_size + (t * kTile) % p.block_size) * kRecord;
+                    bulk_load_hint(st, p.k + o, kKvBytes, &sm.full[stage], pol);
+                    bulk_load_hint(st + kKvBytes, p.v + o, kKvBytes, &sm.full[stage], pol);
+                }
+                if (first_flag) {
+                    const uint16_t* qsrc = p.q + int64_t(b) * p.lq * p.q_stride + int64_t(h) * p.group * kD;
+                    for (int j = 0; j < p.lq; ++j)
+                        bulk_load(sm.qbuf[qb] + j * q_bytes, qsrc + int64_t(j) * p.q_stride, q_bytes, &sm.full[stage]);
+                }
+                ++fills;
+                if (++stage == kStages) { stage = 0; phase ^= 1; }
+                first_flag = last ? kFirst : 0;
+                if (last) qb ^= 1;
+                b = b2, h = h2, t = t2, nt = nt2, ctx = ctx2, at = at2, blk = blk2;
             }
             if (ok) {
                 if (mbar_wait(&sm.empty[stage], phase ^ 1, p.wait_ns)) {
-                    sm.hdr[stage].item = -1;  // sentinel: no more tiles
+                    sm.hdr[stage].tile = -1;  // sentinel: no more tiles
                     mbar_arrive(&sm.full[stage]);
                 } else {
-                    atomicOr(&p.ctrl[2], DEV_ERR_WAIT_EMPTY);
                     ok = false;
                 }
             }
             if (!ok) {
+                atomicOr(p.error, DEV_ERR_WAIT_EMPTY);
                 // Error path: wait (bounded) for every copy still in flight before the CTA's
                 // shared memory is released.
-                for (int s = 0; s < NS; ++s) {
+                for (int s = 0; s < kStages; ++s) {
                     if (fills <= s) break;
-                    const int64_t last = s + ((fills - 1 - s) / NS) * NS;
-                    if (!mbar_wait(&sm.full[s], uint32_t((last / NS) & 1), p.wait_ns))
-                        atomicOr(&p.ctrl[2], DEV_ERR_WAIT_DRAIN);
+                    const int f = s + ((fills - 1 - s) / kStages) * kStages;
+                    if (!mbar_wait(&sm.full[s], uint32_t((f / kStages) & 1), p.wait_ns)) atomicOr(p.error, DEV_ERR_WAIT_DRAIN);
                 }
             }
         }
         __syncwarp();
-    } else {
-        // ------------------------------------------------------------ consumers
-        const int g = lane >> 2, c = lane & 3;
-        // Byte offset in a stage of the 16-byte row this lane hands to ldmatrix: token (lane & 7) of
-        // the warp's 16, group lane >> 3; and of the parameters of token g.
-        const uint32_t frag_off = uint32_t(warp * 16 + (lane & 7)) * kRecord + (lane >> 3) * 16;
-        const uint32_t par_off = uint32_t(warp * 16 + g) * kRecord + q4::kParams;
-        int stage = 0;
-        uint32_t phase = 0, cphase = 0;
-        // Query rows 8 nt + 2 c + j: reference r (log2), sum l, score factor f, group sums of q, limits.
-        float r_ref[NT][2], l_run[NT][2], fac[NT][2], qsum[kGroups][NT][2];
-        int lim[NT][2];
-        int lim_min = 0;
-        float o[kGroups][2][NT][4];   // O^T fragments: 16 dims x 8 rows, in units of 2^-24 and 2^-20
-        float om[kGroups][NT][2];     // sum_t p m of this lane's tokens
-        uint32_t qf[kGroups][2][NT][2];
-        int ev = kExpMin;             // E
-        float s_lim = 0.f;
-        while (true) {
-            // Exit decisions are warp-uniform (the lanes' waits can disagree at the limit).
-            if (!__all_sync(0xffffffffu, mbar_wait(&sm.full[stage], phase, p.wait_ns))) {
-                atomicOr(&p.ctrl[2], DEV_ERR_WAIT_FULL);
-                *reinterpret_cast<volatile int32_t*>(&sm.err) = 1;
-                break;
-            }
+        return;
+    }
+
+    // ---------------------------------------------------------------- consumers
+    const int g = lane >> 2, c = lane & 3;
+    const int row_base = 8 * (warp / C::kSlices);         // this warp's query rows
+    const int tok_warp = (warp % C::kSlices) * C::kWarpTokens;
+    const int rows = min(8, p.rows - row_base);           // of them, those that exist
+    // Byte offsets in a sub-tile's records: the rows this lane hands to ldmatrix (token lane & 7, group
+    // lane >> 3; the parameters of token lane & 15; transposed, those of token (lane & 7) + 8 (lane >> 4)
+    // or a row of ones), the parameters of token g, and those this lane looks over.
+    const uint32_t frag_off = uint32_t(lane & 7) * kRecord + (lane >> 3) * 16;
+    const uint32_t par_off = uint32_t(g) * kRecord + q4::kParams;
+    const uint32_t word_off = uint32_t(lane & 15) * kRecord + q4::kParams;
+    const uint32_t trans_off = uint32_t((lane & 7) + (lane >> 4) * 8) * kRecord + q4::kParams;
+    const uint32_t look_off = uint32_t(lane) * kRecord + q4::kParams;
+    constexpr uint32_t kLo = 0x000f000fu, kHi = 0x00f000f0u;
+    int stage = 0;
+    uint32_t phase = 0, cphase = 0;
+    // Query rows 2 c + e: reference (log2), factor of the scores, limit.
+    float r_ref[2], f_row[2];
+    int lim[2];
+    int lim_min = 0;
+    uint32_t qf[kGroups][2][2], qs[2];  // B operands of row g: q, and (0, sum q) of group c
+    // O^T fragments (16 dims x 8 rows in units of 2^-24), and the product with the parameter words:
+    // its row g is sum_t p * (half-word g), rows 8.. are sum_t p.
+    float o[kGroups][2][4], om[4];
+    float y_lim = 0.f, s_lim = 0.f;  // kLazyMax - E, and the value scale that E allows
+    bool reading = false;            // the last combine's shared memory may still be read by other warps
+    while (true) {
+        // Exit decisions are warp-uniform (the lanes' waits can disagree at the limit).
+        if (!__all_sync(0xffffffffu, mbar_wait(&sm.full[stage], phase, p.wait_ns))) {
+            atomicOr(p.error, DEV_ERR_WAIT_FULL);
+            *reinterpret_cast<volatile int32_t*>(&sm.err) = 1;
+            break;
+        }
+        const int tile = sm.hdr[stage].tile, flags = sm.hdr[stage].flags, ctx = sm.hdr[stage].ctx;
+        // Votes tell the compiler that these branches are uniform.
+        if (__any_sync(0xffffffffu, tile < 0)) break;
+        if (__any_sync(0xffffffffu, flags & kFirst)) {
             // A sibling consumer warp that gave up will not reach the consumer barrier below.
             if (__any_sync(0xffffffffu, *reinterpret_cast<volatile int32_t*>(&sm.err) != 0)) break;
-            const Header hd = sm.hdr[stage];
-            if (hd.item < 0) break;
-            if (hd.flags & kFirst) {
+            const uint8_t* qrow = sm.qbuf[flags & kQBuf ? 1 : 0] + (row_base + g) * kD * 2;
+            float x[kGroups][8];
+            float mx = 0.f;
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    const int row = 8 * nt + g;
-                    float x[kGroups][8];
-                    float mx = 0.f;
+            for (int j = 0; j < kGroups; ++j) {
+                uint4 w = make_uint4(0, 0, 0, 0);
+                if (g < rows) w = *reinterpret_cast<const uint4*>(qrow + (32 * j + 8 * c) * 2);
+                const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-                    for (int j = 0; j < kGroups; ++j) {
-                        uint4 w = make_uint4(0, 0, 0, 0);
-                        if (row < p.rows)
-                            w = *reinterpret_cast<const uint4*>(sm.qbuf[stage] + row * kD * 2 + (32 * j + 8 * c) * 2);
-                        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            x[j][2 * i] = lo_f<BF16>(u[i]);
-                            x[j][2 * i + 1] = hi_f<BF16>(u[i]);
-                            mx = fmaxf(mx, fmaxf(fabsf(x[j][2 * i]), fabsf(x[j][2 * i + 1])));
-                        }
-                    }
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                    // The row times 2^-eq has its largest element in [2^13, 2^14).
-                    const int eq = mx > 0.f ? min(max((__float_as_int(mx) >> 23) - 127 - 13, kExpMin), kExpMax) : 0;
-                    const float sc = exp2_int(-eq);
-                    float sum[kGroups];
-#pragma unroll
-                    for (int j = 0; j < kGroups; ++j) {
-                        sum[j] = 0.f;
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            x[j][i] *= sc;
-                            sum[j] += x[j][i];
-                        }
-                        sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], 1);
-                        sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], 2);
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            qf[j][i][nt][0] = pack2<false>(x[j][4 * i], x[j][4 * i + 1]);
-                            qf[j][i][nt][1] = pack2<false>(x[j][4 * i + 2] * 0.0625f, x[j][4 * i + 3] * 0.0625f);
-                        }
-                    }
-                    const float f = p.scale_log2 * exp2_int(eq + 24);
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int src = (2 * c + e) * 4;  // a lane that holds query row 8 nt + 2 c + e
-                        fac[nt][e] = __shfl_sync(0xffffffffu, f, src);
-#pragma unroll
-                        for (int j = 0; j < kGroups; ++j)
-                            qsum[j][nt][e] = __shfl_sync(0xffffffffu, sum[j], src) * 5.9604644775390625e-8f;  // 2^-24
-                        const int rw = 8 * nt + 2 * c + e;
-                        // Padding rows (past p.rows) see the whole context: only rows that exist mask.
-                        lim[nt][e] = rw < p.rows ? hd.ctx - p.lq + rw / p.group : hd.ctx - 1;
-                        r_ref[nt][e] = kNone;
-                        l_run[nt][e] = 0.f;
-                    }
+                for (int i = 0; i < 4; ++i) {
+                    x[j][2 * i] = lo_f<BF16>(u[i]);
+                    x[j][2 * i + 1] = hi_f<BF16>(u[i]);
+                    mx = max3f(mx, fabsf(x[j][2 * i]), fabsf(x[j][2 * i + 1]));
                 }
-                lim_min = hd.ctx - p.lq;  // row 0's limit, the smallest
-                ev = kExpMin;
-                s_lim = 0.f;
-#pragma unroll
-                for (int j = 0; j < kGroups; ++j)
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        om[j][nt][0] = om[j][nt][1] = 0.f;
-#pragma unroll
-                        for (int t = 0; t < 2; ++t)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) o[j][t][nt][e] = 0.f;
-                    }
             }
-            const int tok_base = hd.tile * kTile + warp * 16;
-            uint8_t* st = sm.stages[stage];
-            bool wrote = false;
-            if (tok_base < hd.ctx) {
-                // Records past the context may hold anything (a NaN scale times a probability of 0 is
-                // NaN), a page outside the cache was not loaded: both read as zeros.
-                const int first = (hd.flags & kNoPage) ? 0 : hd.ctx - tok_base;
-                if (first < 16) {
-                    for (int i = lane; i < (16 - first) * (kRecord / 16); i += 32) {
-                        const int at = (warp * 16 + first) * kRecord + i * 16;
-                        *reinterpret_cast<uint4*>(st + at) = make_uint4(0, 0, 0, 0);
-                        *reinterpret_cast<uint4*>(st + kKvBytes + at) = make_uint4(0, 0, 0, 0);
-                    }
-                    wrote = true;
-                    __syncwarp();
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            const int eq = mx > 0.f ? min(max((__float_as_int(mx) >> 23) - 127 - 3, -kExpMax), kExpMax) : 0;
+            const float sc = exp2_int(-eq);
+            float mine = 0.f;  // sum(q) of group c
+#pragma unroll
+            for (int j = 0; j < kGroups; ++j) {
+                float sum = 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    x[j][i] *= sc;
+                    sum += x[j][i];
                 }
-                constexpr uint32_t kLo = 0x000f000fu, kHi = 0x00f000f0u;
-                // ---- S^T = K Q^T ----
-                uint32_t ka[kGroups], kb[kGroups];  // word c of tokens g and g + 8
-                ldsm_x4(ka[0], ka[1], ka[2], ka[3], smem_u32(st) + frag_off);
-                ldsm_x4(kb[0], kb[1], kb[2], kb[3], smem_u32(st) + frag_off + 8 * kRecord);
-                const uint4 pka4 = *reinterpret_cast<const uint4*>(st + par_off);
-                const uint4 pkb4 = *reinterpret_cast<const uint4*>(st + par_off + 8 * kRecord);
-                const uint4 pva4 = *reinterpret_cast<const uint4*>(st + kKvBytes + par_off);
-                const uint4 pvb4 = *reinterpret_cast<const uint4*>(st + kKvBytes + par_off + 8 * kRecord);
-                const uint32_t pka[4] = {pka4.x, pka4.y, pka4.z, pka4.w}, pkb[4] = {pkb4.x, pkb4.y, pkb4.z, pkb4.w};
-                float x[NT][4];
+                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                if (c == j) mine = sum;
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) x[nt][0] = x[nt][1] = x[nt][2] = x[nt][3] = 0.f;
-#pragma unroll
-                for (int j = 0; j < kGroups; ++j) {
-                    const uint32_t a0[4] = {ka[j] & kLo, kb[j] & kLo, ka[j] & kHi, kb[j] & kHi};
-                    const uint32_t wa = ka[j] >> 8, wb = kb[j] >> 8;
-                    const uint32_t a1[4] = {wa & kLo, wb & kLo, wa & kHi, wb & kHi};
-                    const float sa = lo_f<BF16>(pka[j]), ma = hi_f<BF16>(pka[j]);
-                    const float sb = lo_f<BF16>(pkb[j]), mb = hi_f<BF16>(pkb[j]);
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        float acc[4] = {0.f, 0.f, 0.f, 0.f};
-                        mma_16816<false>(acc, a0, qf[j][0][nt][0], qf[j][0][nt][1]);
-                        mma_16816<false>(acc, a1, qf[j][1][nt][0], qf[j][1][nt][1]);
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            x[nt][e] = fmaf(sa, acc[e], fmaf(ma, qsum[j][nt][e], x[nt][e]));
-                            x[nt][2 + e] = fmaf(sb, acc[2 + e], fmaf(mb, qsum[j][nt][e], x[nt][2 + e]));
-                        }
-                    }
+                for (int i = 0; i < 2; ++i) {
+                    qf[j][i][0] = pack2<false>(x[j][4 * i], x[j][4 * i + 1]);
+                    qf[j][i][1] = pack2<false>(x[j][4 * i + 2] * 0.0625f, x[j][4 * i + 3] * 0.0625f);
                 }
-                // ---- log2 probabilities, masks, running references ----
-                const bool edge = tok_base + 15 > lim_min;  // the tile reaches past some row's last visible token
+            }
+            split2<BF16>(make_float2(0.f, mine), qs[0], qs[1]);
+            const float fm = p.scale_log2 * exp2_int(eq);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+            for (int e = 0; e < 2; ++e) {
+                const int rw = 2 * c + e;
+                f_row[e] = __shfl_sync(0xffffffffu, fm, rw * 4);  // a lane of row rw
+                // Padding rows see the whole context: only rows that exist mask.
+                lim[e] = rw < rows ? ctx - p.lq + (((row_base + rw) * p.group_inv) >> 16) : ctx - 1;
+                r_ref[e] = kNone;
+            }
+            lim_min = ctx - p.lq + ((row_base * p.group_inv) >> 16);  // the smallest: the first row's
+            y_lim = kLazyMax - float(kExpMin<BF16>);
+            s_lim = 0.f;
+            om[0] = om[1] = om[2] = om[3] = 0.f;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) x[nt][e] *= fac[nt][e & 1];
-                if (edge) {
+            for (int j = 0; j < kGroups; ++j)
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
+                for (int t = 0; t < 2; ++t)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (tok_base + g + (e >> 1) * 8 > lim[nt][e & 1]) x[nt][e] = -INFINITY;
+                    for (int e = 0; e < 4; ++e) o[j][t][e] = 0.f;
+        }
+        bool wrote = false;
+        {
+            // Records past the context may hold anything (a NaN scale times a probability of 0 is
+            // NaN), a page outside the cache was not loaded: both read as zeros.
+            const int left = ctx - (tile * kTile + tok_warp);
+            const int first = (flags & kNoPage) ? 0 : left;
+            if (__any_sync(0xffffffffu, left > 0 && first < C::kWarpTokens)) {
+                for (int i = lane; i < (C::kWarpTokens - first) * (kRecord / 16); i += 32) {
+                    uint8_t* at = sm.stages[stage] + (tok_warp + first) * kRecord + i * 16;
+                    *reinterpret_cast<uint4*>(at) = make_uint4(0, 0, 0, 0);
+                    *reinterpret_cast<uint4*>(at + kKvBytes) = make_uint4(0, 0, 0, 0);
                 }
-                float sva[4], svb[4], mva[4], mvb[4];
+                // Where two warps share a slice (9 to 16 rows) each clears it for itself, with the same zeros.
+                wrote = true;
+                __syncwarp();
+            }
+        }
+#pragma unroll 1
+        for (int sub = 0; sub < C::kWarpTokens; sub += 32) {
+            const int tok_base = tile * kTile + tok_warp + sub;
+            if (__any_sync(0xffffffffu, tok_base >= ctx)) break;
+            // Two copies of the step, so that the common one is straight code: EDGE is a step that reaches past
+            // some row's last visible token.
+            auto step = [&](auto edge) {
+            constexpr bool EDGE = decltype(edge)::value;
+            uint8_t* kb = sm.stages[stage] + (tok_warp + sub) * kRecord;
+            uint8_t* vb = kb + kKvBytes;
+            // ---- log2 scores x: codes and minima of S^T = K Q^T ----
+            float x[2][4];  // sub-tile of 16: token g (+ 8 for e >= 2), rows 2 c, 2 c + 1
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const uint8_t* ks = kb + u * 16 * kRecord;
+                uint32_t kw[2][kGroups];  // word c of token g (g + 8)
+                ldsm_x4(kw[0][0], kw[0][1], kw[0][2], kw[0][3], smem_u32(ks) + frag_off);
+                ldsm_x4(kw[1][0], kw[1][1], kw[1][2], kw[1][3], smem_u32(ks) + frag_off + 8 * kRecord);
+                const uint4 pa4 = *reinterpret_cast<const uint4*>(ks + par_off);
+                const uint4 pb4 = *reinterpret_cast<const uint4*>(ks + par_off + 8 * kRecord);
+                float xm[4];
                 {
-                    const uint32_t pa[4] = {pva4.x, pva4.y, pva4.z, pva4.w}, pb[4] = {pvb4.x, pvb4.y, pvb4.z, pvb4.w};
-#pragma unroll
-                    for (int j = 0; j < kGroups; ++j) {
-                        sva[j] = lo_f<BF16>(pa[j]);
-                        mva[j] = hi_f<BF16>(pa[j]);
-                        svb[j] = lo_f<BF16>(pb[j]);
-                        mvb[j] = hi_f<BF16>(pb[j]);
-                    }
+                    uint32_t a[4];  // word c of tokens g, g + 8, g, g + 8
+                    ldsm_x4(a[0], a[1], a[2], a[3], smem_u32(ks) + word_off);
+                    mma_zero<BF16>(xm, a, qs[0], qs[1]);
                 }
-                const float s_max = fmaxf(max3f(max3f(sva[0], sva[1], sva[2]), sva[3], svb[0]), max3f(svb[1], svb[2], svb[3]));
-                float y_max = -INFINITY;
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) y_max = fmaxf(y_max, x[nt][e] - r_ref[nt][e & 1]);
-                if (__any_sync(0xffffffffu, y_max > kLazyMax - float(ev) || s_max > s_lim)) {
-                    // Rare: raise E to the value scales of this tile, the rows' maxima to its scores.
-                    float sm_all = s_max;
-#pragma unroll
-                    for (int sh = 1; sh <= 16; sh <<= 1) sm_all = fmaxf(sm_all, __shfl_xor_sync(0xffffffffu, sm_all, sh));
-                    int raise = 0;
-                    if (sm_all > s_lim) {
-                        const int en = min(max((__float_as_int(sm_all) >> 23) - 127 - 2, ev), kExpMax);
-                        raise = en - ev;
-                        ev = en;
-                        s_lim = en == kExpMax ? INFINITY : exp2_int(en + 7);
-                    }
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            float tm = fmaxf(x[nt][e], x[nt][2 + e]);
-#pragma unroll
-                            for (int sh = 4; sh <= 16; sh <<= 1) tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, sh));
-                            const float ro = r_ref[nt][e];
-                            const float rn = fmaxf(ro == kNone ? kNone : ro + float(raise), tm == -INFINITY ? kNone : tm + float(ev));
-                            const float alpha = ro == kNone ? 0.f : fast_exp2(ro - rn);
-                            r_ref[nt][e] = rn;
-                            l_run[nt][e] *= alpha;
-#pragma unroll
-                            for (int j = 0; j < kGroups; ++j) {
-                                om[j][nt][e] *= alpha;
-#pragma unroll
-                                for (int t = 0; t < 2; ++t) {
-                                    o[j][t][nt][e] *= alpha;
-                                    o[j][t][nt][2 + e] *= alpha;
-                                }
-                            }
-                        }
-                }
-                float pr[NT][4];
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) pr[nt][e] = fast_exp2(x[nt][e] - r_ref[nt][e & 1]);
-                    l_run[nt][0] += pr[nt][0] + pr[nt][2];
-                    l_run[nt][1] += pr[nt][1] + pr[nt][3];
-                }
-                if (edge) {
-                    // A stored non-finite value (s = m = NaN) counts for the rows that see its token only.
-#pragma unroll
-                    for (int j = 0; j < kGroups; ++j) {
-                        const bool bad_a = !(fabsf(sva[j]) <= FLT_MAX && fabsf(mva[j]) <= FLT_MAX);
-                        const bool bad_b = !(fabsf(svb[j]) <= FLT_MAX && fabsf(mvb[j]) <= FLT_MAX);
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                            for (int e = 0; e < 2; ++e)
-                                if ((bad_a && pr[nt][e] != 0.f) || (bad_b && pr[nt][2 + e] != 0.f))
-                                    om[j][nt][e] = __int_as_float(0x7fffffff);
-                        if (bad_a) sva[j] = mva[j] = 0.f;
-                        if (bad_b) svb[j] = mvb[j] = 0.f;
-                    }
-                }
-                // ---- O^T += V^T (P s)^T, and the minima's part ----
-                uint32_t va[kGroups], vb[kGroups];  // half-word g of tokens 2 c, 2 c + 1 (va) and 2 c + 8, 2 c + 9 (vb)
-                ldsm_x4_t(va[0], va[1], va[2], va[3], smem_u32(st) + kKvBytes + frag_off);
-                ldsm_x4_t(vb[0], vb[1], vb[2], vb[3], smem_u32(st) + kKvBytes + frag_off + 8 * kRecord);
+                const uint32_t pa[4] = {pa4.x, pa4.y, pa4.z, pa4.w}, pb[4] = {pb4.x, pb4.y, pb4.z, pb4.w};
 #pragma unroll
                 for (int j = 0; j < kGroups; ++j) {
-                    uint32_t b[NT][2];
+                    const uint32_t wa = kw[0][j], wb = kw[1][j], wa8 = wa >> 8, wb8 = wb >> 8;
+                    const uint32_t a0[4] = {wa & kLo, wb & kLo, wa & kHi, wb & kHi};
+                    const uint32_t a1[4] = {wa8 & kLo, wb8 & kLo, wa8 & kHi, wb8 & kHi};
+                    const float sa = lo_f<BF16>(pa[j]), sb = lo_f<BF16>(pb[j]);
+                    float acc[4];
+                    mma_zero<false>(acc, a0, qf[j][0][0], qf[j][0][1]);
+                    mma<false>(acc, a1, qf[j][1][0], qf[j][1][1]);
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        b[nt][0] = movmatrix_t(pack2<false>(pr[nt][0] * sva[j], pr[nt][1] * sva[j]));
-                        b[nt][1] = movmatrix_t(pack2<false>(pr[nt][2] * svb[j], pr[nt][3] * svb[j]));
+                    for (int e = 0; e < 4; ++e) {
+                        const float sc = e < 2 ? sa : sb;
+                        x[u][e] = j == 0 ? sc * acc[e] : fmaf(sc, acc[e], x[u][e]);
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[u][e] = fmaf(x[u][e], 16777216.f, xm[e]) * f_row[e & 1];
+            }
+            // ---- masks; references ----
+            if constexpr (EDGE) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (tok_base + 16 * u + g + (e >> 1) * 8 > lim[e & 1]) x[u][e] = -INFINITY;
+            }
+            float y_max = -INFINITY;
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                y_max = fmaxf(y_max, max3f(fmaxf(x[0][e], x[0][2 + e]), x[1][e], x[1][2 + e]) - r_ref[e]);
+            const uint4 look = *reinterpret_cast<const uint4*>(vb + look_off);  // value parameters of token `lane`
+            const float s_max = fmaxf(max3f(lo_f<BF16>(look.x), lo_f<BF16>(look.y), lo_f<BF16>(look.z)), lo_f<BF16>(look.w));
+            if (__any_sync(0xffffffffu, y_max > y_lim || s_max > s_lim)) {
+                // Rare: raise E to the value scales of this tile, the rows' maxima to its scores.
+                float sm_all = s_max;
+#pragma unroll
+                for (int sh = 1; sh <= 16; sh <<= 1) sm_all = fmaxf(sm_all, __shfl_xor_sync(0xffffffffu, sm_all, sh));
+                float raise = 0.f;
+                if (sm_all > s_lim) {
+                    const int old = int(kLazyMax - y_lim);  // E
+                    const int en = min(max((__float_as_int(sm_all) >> 23) - 127 - 2, old), kExpMax);
+                    raise = float(en - old);
+                    y_lim = kLazyMax - float(en);
+                    s_lim = en == kExpMax ? INFINITY : exp2_int(en + 7);
+                }
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float tm = max3f(fmaxf(x[0][e], x[0][2 + e]), x[1][e], x[1][2 + e]);
+#pragma unroll
+                    for (int sh = 4; sh <= 16; sh <<= 1) tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, sh));
+                    const float ro = r_ref[e];
+                    const float rn = fmaxf(ro == kNone ? kNone : ro + raise, tm == -INFINITY ? kNone : tm + (kLazyMax - y_lim));
+                    const float alpha = ro == kNone ? 0.f : fast_exp2(ro - rn);
+                    r_ref[e] = rn;
+                    om[e] *= alpha;
+                    om[2 + e] *= alpha;
+#pragma unroll
+                    for (int j = 0; j < kGroups; ++j)
+#pragma unroll
+                        for (int t = 0; t < 2; ++t) {
+                            o[j][t][e] *= alpha;
+                            o[j][t][2 + e] *= alpha;
+                        }
+                }
+            }
+            if constexpr (EDGE) {
+                // A stored non-finite value (s = m = NaN) counts for the rows that see its token only: it
+                // becomes a NaN of their sums here, and a zero as an operand below.
+                const uint32_t lw[4] = {look.x, look.y, look.z, look.w};
+#pragma unroll
+                for (int j = 0; j < kGroups; ++j) {
+                    const bool mine = !(fabsf(lo_f<BF16>(lw[j])) <= FLT_MAX && fabsf(hi_f<BF16>(lw[j])) <= FLT_MAX);
+                    uint32_t bad = __ballot_sync(0xffffffffu, mine);
+                    for (; bad; bad &= bad - 1) {
+                        const int t = tok_base + __ffs(bad) - 1;
 #pragma unroll
                         for (int e = 0; e < 2; ++e)
-                            om[j][nt][e] = fmaf(pr[nt][e], mva[j], fmaf(pr[nt][2 + e], mvb[j], om[j][nt][e]));
+                            if (g == 2 * j + 1 && t <= lim[e]) om[e] = __int_as_float(0x7fffffff);
+                    }
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const uint8_t* vs = vb + u * 16 * kRecord;
+                float y[4];  // probabilities
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[e] = fast_exp2(x[u][e] - r_ref[e & 1]);
+                // ---- sum_t p (parameter words), sum_t p ----
+                {
+                    uint32_t pt[4];  // half-word g of tokens 2 c, 2 c + 1 (+ 8); ones
+                    ldsm_x4_t(pt[0], pt[1], pt[2], pt[3], (lane & 8) ? smem_u32(sm.ones) : smem_u32(vs) + trans_off);
+                    if constexpr (EDGE) {
+                        pt[0] = finite2<BF16>(pt[0]);
+                        pt[2] = finite2<BF16>(pt[2]);
+                    }
+                    uint32_t hi[2], lo[2];
+                    split2<BF16>(make_float2(y[0], y[1]), hi[0], lo[0]);
+                    split2<BF16>(make_float2(y[2], y[3]), hi[1], lo[1]);
+                    mma<BF16>(om, pt, transpose8(hi[0]), transpose8(hi[1]));
+                    mma<BF16>(om, pt, transpose8(lo[0]), transpose8(lo[1]));
+                }
+                // ---- O^T += V^T (P s)^T ----
+                uint32_t vw[2][kGroups];  // half-word g of tokens 2 c, 2 c + 1 (+ 8)
+                ldsm_x4_t(vw[0][0], vw[0][1], vw[0][2], vw[0][3], smem_u32(vs) + frag_off);
+                ldsm_x4_t(vw[1][0], vw[1][1], vw[1][2], vw[1][3], smem_u32(vs) + frag_off + 8 * kRecord);
+                const uint4 pa4 = *reinterpret_cast<const uint4*>(vs + par_off);
+                const uint4 pb4 = *reinterpret_cast<const uint4*>(vs + par_off + 8 * kRecord);
+                uint32_t pa[4] = {pa4.x, pa4.y, pa4.z, pa4.w}, pb[4] = {pb4.x, pb4.y, pb4.z, pb4.w};
+                if constexpr (EDGE) {
+#pragma unroll
+                    for (int j = 0; j < kGroups; ++j) {
+                        pa[j] = finite2<BF16>(pa[j]);
+                        pb[j] = finite2<BF16>(pb[j]);
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < kGroups; ++j) {
+                    uint32_t b[2], bl[2];
+                    const float sa = lo_f<BF16>(pa[j]), sb = lo_f<BF16>(pb[j]);
+                    const float2 p0 = make_float2(y[0] * sa, y[1] * sa), p1 = make_float2(y[2] * sb, y[3] * sb);
+                    if constexpr (BF16) {
+                        b[0] = transpose8(pack2<false>(p0.x, p0.y));
+                        b[1] = transpose8(pack2<false>(p1.x, p1.y));
+                    } else {
+                        uint32_t hi[2], lo[2];
+                        split2<false>(p0, hi[0], lo[0]);
+                        split2<false>(p1, hi[1], lo[1]);
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            b[i] = transpose8(hi[i]);
+                            bl[i] = transpose8(lo[i]);
+                        }
                     }
 #pragma unroll
                     for (int t = 0; t < 2; ++t) {
-                        const uint32_t wa = va[j] >> (8 * t), wb = vb[j] >> (8 * t);
-                        const uint32_t a[4] = {wa & kLo, wa & kHi, wb & kLo, wb & kHi};
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) mma_16816<false>(o[j][t][nt], a, b[nt][0], b[nt][1]);
+                        // Bytes n + 16 n' (n' the next nibble) and their low nibbles n: one operation each.
+                        const uint32_t w0 = t ? __byte_perm(vw[0][j], 0, 0x4341) : vw[0][j] & 0x00ff00ffu;
+                        const uint32_t w1 = t ? __byte_perm(vw[1][j], 0, 0x4341) : vw[1][j] & 0x00ff00ffu;
+                        const uint32_t a[4] = {w0 & kLo, w0, w1 & kLo, w1};
+                        mma<false>(o[j][t], a, b[0], b[1]);
+                        if constexpr (!BF16) mma<false>(o[j][t], a, bl[0], bl[1]);
                     }
                 }
             }
-            if (wrote) fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sm.empty[stage]);
-            if (++stage == NS) { stage = 0; phase ^= 1; }
-
-            if (hd.flags & kLast) {
-                // ---- combine the eight warps' states of this item ----
-                // Sums over the lanes that hold the same rows (all g), then O = 2^24 o + sum p m.
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-#pragma unroll
-                        for (int sh = 4; sh <= 16; sh <<= 1)
-                            l_run[nt][e] += __shfl_xor_sync(0xffffffffu, l_run[nt][e], sh);
-#pragma unroll
-                        for (int j = 0; j < kGroups; ++j) {
-#pragma unroll
-                            for (int sh = 4; sh <= 16; sh <<= 1)
-                                om[j][nt][e] += __shfl_xor_sync(0xffffffffu, om[j][nt][e], sh);
-#pragma unroll
-                            for (int t = 0; t < 2; ++t) {
-                                o[j][t][nt][e] = fmaf(o[j][t][nt][e], 16777216.f, om[j][nt][e]);
-                                o[j][t][nt][2 + e] = fmaf(o[j][t][nt][2 + e], 1048576.f, om[j][nt][e]);
-                            }
-                        }
-                    }
-                constexpr int kHalf = kConsumerWarps / 2;
-                // Dimension of o[j][t][.][e] for e < 2; e >= 2 is the next nibble, two dimensions on.
-                const int d0 = 8 * (g >> 1) + (g & 1);
-                // 8 -> 4: warps 4-7 hand their state to warps 0-3, which merge it in registers.
-                if (warp >= kHalf) {
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const int r = 8 * nt + 2 * c + e;
-                            if (g == 0) {
-                                sm.cm[warp][r] = r_ref[nt][e];
-                                sm.cl[warp][r] = l_run[nt][e];
-                            }
-#pragma unroll
-                            for (int j = 0; j < kGroups; ++j)
-#pragma unroll
-                                for (int t = 0; t < 2; ++t) {
-                                    float* cp = &sm.co[warp - kHalf][r][32 * j + 4 * t + d0];
-                                    cp[0] = o[j][t][nt][e];
-                                    cp[2] = o[j][t][nt][2 + e];
-                                }
-                        }
-                }
-                if (!consumer_sync(&sm.cbar, cphase, p.wait_ns)) {
-                    atomicOr(&p.ctrl[2], DEV_ERR_WAIT_PEER);
-                    *reinterpret_cast<volatile int32_t*>(&sm.err) = 1;
-                    break;
-                }
-                if (warp < kHalf) {
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const int r = 8 * nt + 2 * c + e;
-                            const float mb = sm.cm[warp + kHalf][r], lb = sm.cl[warp + kHalf][r];
-                            const float M = fmaxf(r_ref[nt][e], mb);
-                            const float wa = fast_exp2(r_ref[nt][e] - M), wb = fast_exp2(mb - M);
-#pragma unroll
-                            for (int j = 0; j < kGroups; ++j)
-#pragma unroll
-                                for (int t = 0; t < 2; ++t) {
-                                    float* cp = &sm.co[warp][r][32 * j + 4 * t + d0];
-                                    cp[0] = o[j][t][nt][e] * wa + cp[0] * wb;
-                                    cp[2] = o[j][t][nt][2 + e] * wa + cp[2] * wb;
-                                }
-                            if (g == 0) {
-                                sm.cm[warp][r] = M;
-                                sm.cl[warp][r] = l_run[nt][e] * wa + lb * wb;
-                            }
-                        }
-                }
-                if (!consumer_sync(&sm.cbar, cphase, p.wait_ns)) {
-                    atomicOr(&p.ctrl[2], DEV_ERR_WAIT_PEER);
-                    *reinterpret_cast<volatile int32_t*>(&sm.err) = 1;
-                    break;
-                }
-                // 4 -> 1 over shared memory, one output element per thread and round.
-                const bool single = hd.nchunks == 1;
-                const int nel = p.rows * kD;
-                const int cslot = hd.item / p.hkv;  // this chunk's partial slot (before x Hkv + h)
-                for (int idx = tid; idx < nel; idx += kConsumers) {
-                    const int r = idx >> 7, d = idx & (kD - 1);
-                    float M = sm.cm[0][r];
-#pragma unroll
-                    for (int w = 1; w < kHalf; ++w) M = fmaxf(M, sm.cm[w][r]);
-                    float den = 0.f, acc = 0.f;
-#pragma unroll
-                    for (int w = 0; w < kHalf; ++w) {
-                        const float sc = fast_exp2(sm.cm[w][r] - M);
-                        den = fmaf(sm.cl[w][r], sc, den);
-                        acc = fmaf(sm.co[w][r][d], sc, acc);
-                    }
-                    const float val = den == 0.f ? 0.f : acc / den;  // 0: the row sees no token of this item
-                    if (single) {
-                        const int j = r / p.group, gq = r - j * p.group;
-                        p.out[((int64_t(hd.b) * p.lq + j) * p.hq + hd.h * p.group + gq) * kD + d] = to_bits16<BF16>(val);
-                    } else {
-                        const int64_t it = int64_t(cslot) * p.hkv + hd.h;
-                        p.part_o[(it * p.rows + r) * kD + d] = val;
-                        // A NaN sum is handed on as an infinite weight: the merge's maximum skips NaN.
-                        if (d == 0)
-                            p.part_lse[it * p.rows + r] =
-                                den == 0.f ? -INFINITY : (den <= FLT_MAX ? M + fast_log2(den) : INFINITY);
-                    }
-                }
-                if (!single) {
-                    // Publish this chunk (one release fence per CTA, cumulative over the barrier), then
-                    // count it; the last chunk's CTA merges.
-                    if (!consumer_sync(&sm.cbar, cphase, p.wait_ns)) {
-                        atomicOr(&p.ctrl[2], DEV_ERR_WAIT_PEER);
-                        *reinterpret_cast<volatile int32_t*>(&sm.err) = 1;
-                        break;
-                    }
-                    if (tid == 0) {
-                        __threadfence();
-                        const int prev = atomicAdd(&p.counters[hd.b * p.hkv + hd.h], 1);
-                        const bool last = prev == hd.nchunks - 1;
-                        if (last) __threadfence();
-                        sm.flag = last;
-                    }
-                    if (!consumer_sync(&sm.cbar, cphase, p.wait_ns)) {
-                        atomicOr(&p.ctrl[2], DEV_ERR_WAIT_PEER);
-                        *reinterpret_cast<volatile int32_t*>(&sm.err) = 1;
-                        break;
-                    }
-                    if (sm.flag) {
-                        merge_chunks<BF16>(p, hd, pl, tid);
-                        if (tid == 0) p.counters[hd.b * p.hkv + hd.h] = 0;
-                    }
-                }
-                if (!consumer_sync(&sm.cbar, cphase, p.wait_ns)) {
-                    atomicOr(&p.ctrl[2], DEV_ERR_WAIT_PEER);
-                    *reinterpret_cast<volatile int32_t*>(&sm.err) = 1;
-                    break;
-                }
-            }
+            };
+            if (__any_sync(0xffffffffu, tok_base + 31 > lim_min)) step(std::true_type{});
+            else step(std::false_type{});
         }
-    }
+        if (wrote) fence_proxy_async_smem();
+        const Header hd = sm.hdr[stage];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.empty[stage]);
+        if (++stage == kStages) { stage = 0; phase ^= 1; }
+        if (!__any_sync(0xffffffffu, flags & kLast)) continue;
 
-    __syncthreads();
-    if (tid == 0) {
-        __threadfence();
-        const int done = atomicAdd(&p.ctrl[1], 1);
-        if (done == int(gridDim.x) - 1) {
-            // Every CTA has stopped claiming items: re-arm the scheduler.
-            atomicExch(&p.ctrl[0], 0);
-            atomicExch(&p.ctrl[1], 0);
+        // ---- combine the warps' states of this item ----
+        // O = 2^24 o + sum p m; n' is a sixteenth of the byte's sum less the low nibble's.
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int j = 0; j < kGroups; ++j) {
+                const float mj = __shfl_sync(0xffffffffu, om[e], (2 * j + 1) * 4 + c);
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    o[j][t][2 + e] = fmaf(o[j][t][2 + e] - o[j][t][e], 1048576.f, mj);
+                    o[j][t][e] = fmaf(o[j][t][e], 16777216.f, mj);
+                }
+            }
+        // Dimension of o[j][t][e] for e < 2; e >= 2 is the next nibble, two dimensions on.
+        const int d0 = 8 * (g >> 1) + (g & 1);
+        const bool single = hd.nch == 1;
+        const int64_t slot = 2 * int64_t(blockIdx.x) + (int(blockIdx.x) == hd.first ? 1 : 0);
+        const int w0 = (warp / C::kSlices) * C::kSlices;  // first warp of this group of rows
+        bool ok = true;
+#pragma unroll
+        for (int r0 = 0; r0 < 8; r0 += C::kPassRows) {
+            if (r0 >= p.rows || !ok) break;  // the first group's rows: the same passes for all warps
+            const int nr = min(C::kPassRows, rows - r0);
+            if (reading) ok = consumer_wait(&sm.cbar, cphase, p.wait_ns);
+            if (!ok) break;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int r = 2 * c + e - r0;
+                if (r >= 0 && r < nr) {
+                    if (g == 0) {
+                        sm.cm[warp][r] = r_ref[e];
+                        sm.cl[warp][r] = om[2 + e];
+                    }
+#pragma unroll
+                    for (int j = 0; j < kGroups; ++j)
+#pragma unroll
+                        for (int t = 0; t < 2; ++t) {
+                            float* cp = &sm.co[warp][r][32 * j + 4 * t + d0];
+                            cp[0] = o[j][t][e];
+                            cp[2] = o[j][t][2 + e];
+                        }
+                }
+            }
+            mbar_arrive(&sm.cbar);
+            ok = consumer_wait(&sm.cbar, cphase, p.wait_ns);
+            if (!ok) break;
+            // This warp's share of the pass's elements, two neighbours per lane and round.
+            const int n = nr * (kD / C::kSlices);
+            for (int i = 2 * lane; i < n; i += 64) {
+                const int el = (warp - w0) * n + i, r = el >> 7, d = el & (kD - 1);
+                float M = sm.cm[w0][r];
+#pragma unroll
+                for (int w = 1; w < C::kSlices; ++w) M = fmaxf(M, sm.cm[w0 + w][r]);
+                float den = 0.f, a0 = 0.f, a1 = 0.f;
+#pragma unroll
+                for (int w = 0; w < C::kSlices; ++w) {
+                    const float sc = fast_exp2(sm.cm[w0 + w][r] - M);
+                    den = fmaf(sm.cl[w0 + w][r], sc, den);
+                    a0 = fmaf(sm.co[w0 + w][r][d], sc, a0);
+                    a1 = fmaf(sm.co[w0 + w][r][d + 1], sc, a1);
+                }
+                const float inv = den == 0.f ? 0.f : __fdividef(1.f, den);  // 0: the row sees no token of this item
+                const int row = row_base + r0 + r;
+                if (single)
+                    *reinterpret_cast<uint32_t*>(p.out + out_row(p, hd.b, hd.h, row) + d) = pack2<BF16>(a0 * inv, a1 * inv);
+                else
+                    *reinterpret_cast<float2*>(p.part_o + (slot * p.rows + row) * kD + d) = make_float2(a0 * inv, a1 * inv);
+            }
+            if (!single && lane < nr) {
+                float M = sm.cm[w0][lane];
+#pragma unroll
+                for (int w = 1; w < C::kSlices; ++w) M = fmaxf(M, sm.cm[w0 + w][lane]);
+                float den = 0.f;
+#pragma unroll
+                for (int w = 0; w < C::kSlices; ++w) den = fmaf(sm.cl[w0 + w][lane], fast_exp2(sm.cm[w0 + w][lane] - M), den);
+                // A NaN sum is handed on as an infinite weight: the merge's maximum skips NaN.
+                p.part_lse[(slot * kWarps + warp) * p.rows + row_base + r0 + lane] =
+                    den == 0.f ? -INFINITY : (den <= FLT_MAX ? M + fast_log2(den) : INFINITY);
+            }
+            mbar_arrive(&sm.cbar);
+            reading = true;
+        }
+        if (!ok) {
+            atomicOr(p.error, DEV_ERR_WAIT_PEER);
+            *reinterpret_cast<volatile int32_t*>(&sm.err) = 1;
+            break;
+        }
+        if (!single) {
+            // Publish this warp's share of the chunk (one release fence per warp, cumulative over the warp
+            // barrier), then count it; the last chunk's warp of this number merges the share.
+            __syncwarp();
+            int last = 0;
+            int32_t* counter = &p.counters[hd.first * kWarps + warp];
+            if (lane == 0) {
+                __threadfence();
+                last = atomicAdd(counter, 1) == hd.nch - 1;
+                if (last) __threadfence();
+            }
+            if (__shfl_sync(0xffffffffu, last, 0)) {
+                merge_share<BF16, ROWS16>(p, hd, row_base, rows, warp, lane);
+                if (lane == 0) *counter = 0;
+            }
         }
     }
 }
 
-template <bool BF16, int NT>
-void launch(const Q4Params& prm, cudaStream_t s) {
-    const void* fn = (const void*)paged_attention_q4_kernel<BF16, NT>;
-    ensure_smem_attr(fn, int(sizeof(Smem<NT>)));
-    paged_attention_q4_kernel<BF16, NT>
-        <<<device_sm_count() * Cfg<NT>::kCtas, kThreads, sizeof(Smem<NT>), s>>>(prm);
+template <bool BF16, bool ROWS16>
+void launch(const Params& prm, int ctas, cudaStream_t s) {
+    const void* fn = (const void*)paged_attention_q4_kernel<BF16, ROWS16>;
+    ensure_smem_attr(fn, int(sizeof(Smem<ROWS16>)));
+    paged_attention_q4_kernel<BF16, ROWS16><<<ctas, kThreads, sizeof(Smem<ROWS16>), s>>>(prm);
 }
 
 }  // namespace
-}  // namespace pa
+}  // namespace pq4
 }  // namespace b200
+
+extern "C" size_t b200_paged_attention_q4_workspace_size(int32_t query_len, int32_t group_size) {
+    using namespace b200::pq4;
+    if (query_len < 1 || group_size < 1) return 0;
+    const int64_t rows = int64_t(query_len) * group_size;
+    return rows > 16 ? 0 : workspace_bytes(int(rows), grid_ctas());
+}
 
 extern "C" int32_t b200_paged_attention_q4(void* out, const void* q, int64_t q_stride_token, const void* k_cache,
                                            const void* v_cache, int32_t num_blocks, int32_t block_size,
                                            const int32_t* block_tables, int64_t block_table_stride,
-                                           int32_t block_table_width, const int32_t* context_lens, int32_t batch, int32_t query_len,
-                                           int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
-                                           float softmax_scale, int32_t dtype, void* workspace, size_t workspace_bytes,
+                                           int32_t block_table_width, const int32_t* context_lens, int32_t batch,
+                                           int32_t query_len, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                           float softmax_scale, int32_t dtype, void* workspace, size_t workspace_size,
                                            void* stream) {
     using namespace b200;
-    using namespace b200::pa;
+    using namespace b200::pq4;
     clear_error();
     B200_REQUIRE(batch >= 0, "paged_attention_q4: batch %d < 0", batch);
     if (batch == 0) return B200_OK;
@@ -671,61 +897,58 @@ extern "C" int32_t b200_paged_attention_q4(void* out, const void* q, int64_t q_s
     B200_REQUIRE(num_blocks > 0 && int64_t(num_blocks) * block_size < (int64_t(1) << 31),
                  "paged_attention_q4: num_blocks %d out of range", num_blocks);
     B200_REQUIRE(block_table_width > 0 && int64_t(block_table_width) * block_size < (int64_t(1) << 31) &&
-                     block_table_stride >= 0 && block_table_stride <= INT32_MAX,
+                     block_table_stride >= 0,
                  "paged_attention_q4: block table of %d entries, stride %lld out of range", block_table_width,
                  (long long)block_table_stride);
+    if ((int64_t(block_table_width) * (block_size / kTile) + kPairCost) * batch > INT32_MAX / 2 / num_kv_heads)
+        return fail(B200_ERR_UNSUPPORTED, "paged_attention_q4: %d tables of %d blocks of %d tokens", batch,
+                    block_table_width, block_size);
     auto al16 = [](const void* a) { return (reinterpret_cast<uintptr_t>(a) & 15) == 0; };
     B200_REQUIRE(q_stride_token >= int64_t(num_heads) * head_dim && q_stride_token % 8 == 0 && al16(q) && al16(out) &&
                      al16(k_cache) && al16(v_cache),
                  "paged_attention_q4: q, out and the caches must be 16-byte aligned, q token stride (%lld) a multiple of 8 "
                  "and at least Hq*D",
                  (long long)q_stride_token);
-    if (int64_t(batch) * num_kv_heads > kCounterSlots)
-        return fail(B200_ERR_UNSUPPORTED, "paged_attention_q4: batch * num_kv_heads > %d", kCounterSlots);
-    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) || workspace_bytes < kFixedBytes)
+    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) ||
+        workspace_size < workspace_bytes(int(rows), grid_ctas()))
         return fail(B200_ERR_WORKSPACE, "paged_attention_q4: workspace missing, unaligned or smaller than %zu bytes",
-                    kFixedBytes);
-    const int64_t max_items = int64_t(workspace_bytes - kFixedBytes) / (rows * (kD + 1) * 4);
-    if (max_items < int64_t(batch) * num_kv_heads)
-        return fail(B200_ERR_WORKSPACE, "paged_attention_q4: workspace holds %lld items, batch * Hkv = %lld",
-                    (long long)max_items, (long long)batch * num_kv_heads);
+                    workspace_bytes(int(rows), grid_ctas()));
 
-    Q4Params prm;
+    const int ctas = grid_ctas();
+    Params prm;
+    prm.q = static_cast<const uint16_t*>(q);
+    prm.q_stride = q_stride_token;
+    prm.out = static_cast<uint16_t*>(out);
     prm.k = static_cast<const uint8_t*>(k_cache);
     prm.v = static_cast<const uint8_t*>(v_cache);
-    Params& b = prm.base;
-    b.q = static_cast<const uint16_t*>(q);
-    b.q_stride = q_stride_token;
-    b.out = static_cast<uint16_t*>(out);
-    b.block_tables = block_tables;
-    b.bt_stride = int32_t(block_table_stride);
-    b.bt_width = block_table_width;
-    b.context_lens = context_lens;
-    b.batch = batch;
-    b.lq = query_len;
-    b.hq = num_heads;
-    b.hkv = num_kv_heads;
-    b.group = group;
-    b.rows = int32_t(rows);
-    b.block_size = block_size;
-    b.num_blocks = num_blocks;
-    b.scale_log2 = softmax_scale * 1.4426950408889634f;
+    prm.block_tables = block_tables;
+    prm.bt_stride = block_table_stride;
+    prm.bt_width = block_table_width;
+    prm.context_lens = context_lens;
+    prm.batch = batch;
+    prm.lq = query_len;
+    prm.hq = num_heads;
+    prm.hkv = num_kv_heads;
+    prm.group = group;
+    prm.rows = int32_t(rows);
+    prm.block_size = block_size;
+    prm.num_blocks = num_blocks;
+    prm.group_inv = (65536 + group - 1) / group;
+    prm.scale_log2 = softmax_scale * 1.4426950408889634f;
     char* ws = static_cast<char*>(workspace);
-    b.ctrl = reinterpret_cast<int32_t*>(ws);
-    b.counters = reinterpret_cast<int32_t*>(ws + kCtrlWords * 4);
-    b.part_o = reinterpret_cast<float*>(ws + kFixedBytes);
-    b.part_lse = b.part_o + max_items * rows * kD;
-    b.max_items = int32_t(max_items > INT32_MAX / 2 ? INT32_MAX / 2 : max_items);
-    apply_test_hook(b);
+    prm.error = reinterpret_cast<int32_t*>(ws) + 2;
+    prm.counters = reinterpret_cast<int32_t*>(ws + kCtrlBytes);
+    prm.part_o = reinterpret_cast<float*>(ws + fixed_bytes(ctas));
+    prm.part_lse = prm.part_o + size_t(2) * ctas * rows * kD;
+    take_test_hook(&prm.wait_ns, &prm.idle_producer);
 
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const bool wide = rows > 8;
     if (dtype == B200_BF16) {
-        if (wide) launch<true, 2>(prm, s);
-        else launch<true, 1>(prm, s);
+        if (rows > 8) launch<true, true>(prm, ctas, s);
+        else launch<true, false>(prm, ctas, s);
     } else {
-        if (wide) launch<false, 2>(prm, s);
-        else launch<false, 1>(prm, s);
+        if (rows > 8) launch<false, true>(prm, ctas, s);
+        else launch<false, false>(prm, ctas, s);
     }
     B200_CUDA_TRY(cudaGetLastError());
     return B200_OK;

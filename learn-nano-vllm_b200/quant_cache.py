@@ -27,6 +27,7 @@ from .ops import _DTYPES, _require_cuda, _stream
 
 HEAD_DIM = 128
 RECORD_BYTES = 80
+_CONTROL_BYTES = 16384  # covers the control words and counters at the start of an attention workspace
 
 
 def q4_cache_shape(num_blocks: int, block_size: int, num_kv_heads: int, head_dim: int = HEAD_DIM) -> tuple:
@@ -150,28 +151,26 @@ def gather_kvcache_q4(k_cache: torch.Tensor, v_cache: torch.Tensor, cu_seqlens: 
 
 
 # ------------------------------------------------------------------ attention
-_CONTROL_BYTES = 256  # scheduler and error words; one 4-byte counter per (sequence, kv head) follows
 _ws_lock = threading.Lock()
 _workspaces: dict[tuple, torch.Tensor] = {}
 
 
-def q4_workspace_size(query_len: int, group: int, batch_heads: int) -> int:
-    """Bytes of a workspace for calls of up to batch_heads (sequence, kv head) pairs."""
-    # Twice the pairs (a split sequence has at most one remainder beside its full chunks) plus the
-    # items of the waves that the plan aims for (kernel: 3 per CTA, two CTAs per SM).
-    return int(lib().b200_paged_attention_workspace_size(2 * batch_heads + 2048, query_len, group, HEAD_DIM))
+def q4_workspace_size(query_len: int, group: int) -> int:
+    """Bytes of a workspace of `flash_attn_with_kvcache_q4` for query_len * group query rows per kv head
+    (of the current device; it does not depend on the batch)."""
+    return int(lib().b200_paged_attention_q4_workspace_size(query_len, group))
 
 
-def q4_workspace(device, query_len: int, group: int, batch_heads: int) -> torch.Tensor:
-    """Split-K workspace of a call, its control words and counters zero.
+def q4_workspace(device: torch.device, query_len: int, group: int) -> torch.Tensor:
+    """The split-K workspace of a call on the current stream, its control words and counters zero.
 
     Eager calls keep one per (device, stream), grown on demand: calls of one stream run one after
     another and leave it re-armed.  A call that is being captured gets its own from the graph's
     memory pool, zeroed by the graph itself, so that graphs replayed at the same time share nothing."""
-    need = q4_workspace_size(query_len, group, batch_heads)
+    need = q4_workspace_size(query_len, group)
     if torch.cuda.is_current_stream_capturing():
         ws = torch.empty(need, dtype=torch.uint8, device=device)
-        ws[:_CONTROL_BYTES + 4 * batch_heads].zero_()
+        ws[:_CONTROL_BYTES].zero_()
         return ws
     key = (device.index, torch.cuda.current_stream(device).cuda_stream)
     with _ws_lock:
@@ -189,7 +188,7 @@ def flash_attn_with_kvcache_q4(q, k_cache, v_cache, cache_seqlens=None, block_ta
 
     cache_seqlens int32 [B] counts the cached tokens of each row including its Lq queries; rows
     with cache_seqlens <= 0 return zeros.  Tokens whose page lies outside the cache count as zeros.
-    workspace: a caller-owned one of q4_workspace_size(Lq, Hq // Hkv, B * Hkv) bytes, zero-filled
+    workspace: a caller-owned one of q4_workspace_size(Lq, Hq // Hkv) bytes, zero-filled
     once; calls that share it must not overlap (default: one per stream, or per captured call).
     """
     assert cache_seqlens is not None and block_table is not None, "the B200 path reads a paged cache"
@@ -219,7 +218,7 @@ def flash_attn_with_kvcache_q4(q, k_cache, v_cache, cache_seqlens=None, block_ta
     _require_cuda(q, k_cache, v_cache, cache_seqlens, block_table, out)
     scale = D ** -0.5 if softmax_scale is None else softmax_scale
     with torch.cuda.device(q.device):
-        ws = q4_workspace(q.device, Lq, Hq // Hkv, B * Hkv) if workspace is None else workspace
+        ws = q4_workspace(q.device, Lq, Hq // Hkv) if workspace is None else workspace
         rc = lib().b200_paged_attention_q4(out.data_ptr(), q.data_ptr(), q_tok, k_cache.data_ptr(), v_cache.data_ptr(),
                                            k_cache.size(0), k_cache.size(2), block_table.data_ptr(),
                                            block_table.stride(0), block_table.size(1), cache_seqlens.data_ptr(), B, Lq, Hq, Hkv, D,

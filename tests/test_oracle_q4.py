@@ -167,12 +167,12 @@ def test_c_abi_refusals(pkg):
                    (dict(btw=0), ARG), (dict(bts=-1), ARG), (dict(d=96), UNS), (dict(dt=7), UNS)]:
         assert lib.b200_gather_kvcache_q4(*{**ga, **kw}.values()) == rc, kw
     pa = dict(out=a, q=a, qs=512, kc=a, vc=a, nb=1, bs=128, bt=a, bts=1, btw=1, cl=a, b=1, lq=1, hq=4, hkv=2, d=128,
-              sc=0.1, dt=1, ws=a, wb=1 << 20, st=None)
+              sc=0.1, dt=1, ws=a, wb=1 << 24, st=None)
     for kw, rc in [(dict(b=0), 0), (dict(b=-1), ARG), (dict(q=None), ARG), (dict(hq=3), ARG), (dict(hkv=0), ARG),
                    (dict(lq=0), ARG), (dict(lq=9), UNS), (dict(lq=1 << 30), UNS), (dict(d=64), UNS), (dict(dt=2), UNS),
                    (dict(sc=0.0), ARG), (dict(sc=float("nan")), ARG), (dict(sc=float("inf")), ARG), (dict(b=2049), UNS),
                    (dict(bs=64), ARG), (dict(bs=192), ARG), (dict(nb=0), ARG), (dict(btw=0), ARG), (dict(bts=-1), ARG),
                    (dict(btw=1 << 25), ARG), (dict(qs=511), ARG), (dict(qs=516), ARG), (dict(q=a + 8), ARG),
                    (dict(kc=a + 4), ARG), (dict(ws=None), WS), (dict(ws=a + 16), WS), (dict(wb=1024), WS),
-                   (dict(wb=262400), WS)]:
+                   (dict(wb=8192), WS), (dict(b=2048, btw=1 << 22), UNS)]:
         assert lib.b200_paged_attention_q4(*{**pa, **kw}.values()) == rc, (kw, lib.b200_last_error())
