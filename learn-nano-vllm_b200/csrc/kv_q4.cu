@@ -10,8 +10,9 @@
 // head).  A half-warp owns a row (16 bytes, eight dimensions, per lane), so that the four
 // lanes of a quad hold one group: two shuffles find its extremes and every lane ends with one
 // whole word of codes.  The two halves of a warp take the same head of two consecutive tokens,
-// whose records are neighbours in a page (160 bytes, five whole sectors).  A block takes
-// a run of tokens, looks their slots up once and deals the (token pair, row) tasks to its warps.
+// whose records are neighbours in a page (160 bytes, five whole sectors).  A block takes a run
+// of tokens and looks up once where their records lie; each of its warps takes rows (a head's
+// keys or values) and walks the token pairs, kFlight of them in flight.
 #include "kv_q4.cuh"
 
 namespace b200 {
@@ -19,7 +20,8 @@ namespace q4 {
 namespace {
 
 constexpr int kWarps = 8;
-constexpr int kMaxTokens = 32;  // tokens of one block
+constexpr int kMaxTokens = 24;    // tokens of one block
+constexpr int kBlocksPerSm = 4;   // resident (launch bounds)
 
 struct Rows {
     char* k;  // key rows (read by store, written by load and gather)
@@ -34,143 +36,173 @@ struct Cache {
     int64_t num_slots;
 };
 
-__device__ __forceinline__ int64_t record_offset(const Cache& c, int64_t slot, int h) {
+// Byte offset of head 0's record of a slot (heads are block_size records apart).
+__device__ __forceinline__ int64_t record_of(const Cache& c, int32_t slot) {
     const uint32_t blk = uint32_t(slot) / uint32_t(c.block_size);
-    return ((int64_t(blk) * c.hkv + h) * c.block_size + (uint32_t(slot) - blk * c.block_size)) * kRecord;
+    return (int64_t(blk) * c.hkv * c.block_size + (uint32_t(slot) - blk * c.block_size)) * kRecord;
 }
 
-// Runs f(token of the block, row of the token, half-warp lane) over all rows of `count` tokens;
-// both halves of a warp call it together (the token may be past the end: the caller masks it).
-template <typename F>
-__device__ __forceinline__ void for_rows(int count, int rows, F f) {
-    const int lane = threadIdx.x & 31;
-    const int tasks = ((count + 1) / 2) * rows;
-    for (int i = threadIdx.x >> 5; i < tasks; i += kWarps) {
-        const int pair = i / rows;
-        f(2 * pair + (lane >> 4), i - pair * rows, lane & 15);
+// Offsets of a block's tokens that have no record: rows that read as zeros, rows that are left alone.
+constexpr int64_t kZero = -1, kSkip = -2;
+
+// Deals the rows of `count` tokens to the block's warps and calls, kFlight pairs at a time, LOAD and then
+// USE for each: (u, offset of the token's record, the head's records, the lane's 16 bytes of the row).
+// Both halves of a warp run together; past the last pair the offset is kSkip.
+template <int kFlight, typename LOAD, typename USE>
+__device__ __forceinline__ void for_rows(const Rows& rows, const Cache& cache, const int64_t* s_rec, int64_t t0, int count,
+                                         LOAD load, USE use) {
+    const int half = (threadIdx.x >> 4) & 1, l = threadIdx.x & 15, pairs = (count + 1) >> 1;
+    for (int r = blockIdx.y * kWarps + (threadIdx.x >> 5); r < 2 * cache.hkv; r += gridDim.y * kWarps) {
+        const bool v = r >= cache.hkv;
+        const int h = v ? r - cache.hkv : r;
+        const int64_t stride = v ? rows.v_stride : rows.k_stride;
+        char* row = (v ? rows.v : rows.k) + (t0 + half) * stride + h * (kD * 2) + 16 * l;
+        char* records = (v ? cache.v : cache.k) + int64_t(h) * cache.block_size * kRecord;
+        for (int p0 = 0; p0 < pairs; p0 += kFlight) {
+            int64_t rec[kFlight];
+#pragma unroll
+            for (int u = 0; u < kFlight; ++u) {
+                rec[u] = p0 + u < pairs ? s_rec[2 * (p0 + u) + half] : kSkip;
+                load(u, rec[u], records, row + u * 2 * stride);
+            }
+#pragma unroll
+            for (int u = 0; u < kFlight; ++u) use(u, rec[u], records, row + u * 2 * stride);
+            row += kFlight * 2 * stride;
+        }
     }
 }
 
-template <bool BF16, bool VEC>
-__global__ void __launch_bounds__(kWarps * 32)
+template <bool BF16, bool VEC, int kFlight>
+__global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm)
     store_kernel(const Rows rows, const Cache cache, const int32_t* __restrict__ slots, int32_t n, int32_t tokens) {
-    __shared__ int32_t s_slot[kMaxTokens];
+    __shared__ int64_t s_rec[kMaxTokens];
     const int64_t t0 = int64_t(blockIdx.x) * tokens;
     const int count = int(min(int64_t(tokens), n - t0));
     if (threadIdx.x < kMaxTokens) {
         const int32_t s = threadIdx.x < count ? slots[t0 + threadIdx.x] : -1;
-        s_slot[threadIdx.x] = s < cache.num_slots ? s : -1;
+        s_rec[threadIdx.x] = s >= 0 && s < cache.num_slots ? record_of(cache, s) : kSkip;
     }
     __syncthreads();
-    for_rows(count, 2 * cache.hkv, [&](int t, int r, int l) {
-        const bool is_v = r >= cache.hkv;
-        const int h = is_v ? r - cache.hkv : r;
-        const int32_t slot = t < kMaxTokens ? s_slot[t] : -1;
-        uint32_t x[4] = {0, 0, 0, 0};
-        if (slot >= 0) {
-            const char* src = (is_v ? rows.v + (t0 + t) * rows.v_stride : rows.k + (t0 + t) * rows.k_stride) +
-                              (h * kD + 8 * l) * 2;
+    const int l = threadIdx.x & 15;
+    uint32_t x[kFlight][4];
+    for_rows<kFlight>(
+        rows, cache, s_rec, t0, count,
+        [&](int u, int64_t rec, char*, char* row) {
+            x[u][0] = x[u][1] = x[u][2] = x[u][3] = 0;
+            if (rec < 0) return;
             if constexpr (VEC) {
-                const uint4 v = __ldg(reinterpret_cast<const uint4*>(src));
-                x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+                const uint4 w = __ldg(reinterpret_cast<const uint4*>(row));
+                x[u][0] = w.x, x[u][1] = w.y, x[u][2] = w.z, x[u][3] = w.w;
             } else {
-                const uint16_t* e = reinterpret_cast<const uint16_t*>(src);
+                const uint16_t* e = reinterpret_cast<const uint16_t*>(row);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) x[i] = uint32_t(e[2 * i]) | (uint32_t(e[2 * i + 1]) << 16);
+                for (int i = 0; i < 4; ++i) x[u][i] = uint32_t(e[2 * i]) | (uint32_t(e[2 * i + 1]) << 16);
             }
-        }
-        uint32_t params;
-        const uint32_t word = quantise8<BF16>(x, params);
-        if (slot >= 0) {
-            char* rec = (is_v ? cache.v : cache.k) + record_offset(cache, slot, h);
-            *reinterpret_cast<uint32_t*>(rec + 4 * l) = word;
-            if ((l & 3) == 0) *reinterpret_cast<uint32_t*>(rec + kParams + l) = params;
-        }
-    });
+        },
+        [&](int u, int64_t rec, char* records, char*) {
+            uint32_t params;
+            const uint32_t word = quantise8<BF16>(x[u], params);
+            if (rec < 0) return;
+            *reinterpret_cast<uint32_t*>(records + rec + 4 * l) = word;
+            if ((l & 3) == 0) *reinterpret_cast<uint32_t*>(records + rec + kParams + l) = params;
+        });
 }
 
-// Slots of a block's tokens for the readers: kZero for rows that read as zeros, kSkip for rows
-// that are left as they were.
-constexpr int32_t kZero = -1, kSkip = -2;
-
-template <bool BF16, bool VEC>
-__device__ __forceinline__ void read_rows(const Rows& rows, const Cache& cache, const int32_t* s_slot, int64_t t0,
+template <bool BF16, bool VEC, int kFlight>
+__device__ __forceinline__ void read_rows(const Rows& rows, const Cache& cache, const int64_t* s_rec, int64_t t0,
                                           int count) {
-    for_rows(count, 2 * cache.hkv, [&](int t, int r, int l) {
-        const bool is_v = r >= cache.hkv;
-        const int h = is_v ? r - cache.hkv : r;
-        const int32_t slot = t < count ? s_slot[t] : kSkip;
-        if (slot == kSkip) return;
-        uint4 y = make_uint4(0, 0, 0, 0);
-        if (slot >= 0) {
-            const char* rec = (is_v ? cache.v : cache.k) + record_offset(cache, slot, h);
-            y = dequantise8<BF16>(*reinterpret_cast<const uint32_t*>(rec + 4 * l),
-                                  *reinterpret_cast<const uint32_t*>(rec + kParams + (l & ~3)));
-        }
-        char* dst = (is_v ? rows.v + (t0 + t) * rows.v_stride : rows.k + (t0 + t) * rows.k_stride) +
-                    (h * kD + 8 * l) * 2;
-        if constexpr (VEC) {
-            *reinterpret_cast<uint4*>(dst) = y;
-        } else {
-            const uint32_t w[4] = {y.x, y.y, y.z, y.w};
-            uint16_t* e = reinterpret_cast<uint16_t*>(dst);
+    const int l = threadIdx.x & 15;
+    uint32_t word[kFlight], params[kFlight];
+    for_rows<kFlight>(
+        rows, cache, s_rec, t0, count,
+        [&](int u, int64_t rec, char* records, char*) {
+            word[u] = params[u] = 0;
+            if (rec < 0) return;
+            word[u] = __ldg(reinterpret_cast<const uint32_t*>(records + rec + 4 * l));
+            params[u] = __ldg(reinterpret_cast<const uint32_t*>(records + rec + kParams + (l & ~3)));
+        },
+        [&](int u, int64_t rec, char*, char* row) {
+            if (rec == kSkip) return;
+            const uint4 y = dequantise8<BF16>(word[u], params[u]);  // no record: zeros
+            if constexpr (VEC) {
+                *reinterpret_cast<uint4*>(row) = y;
+            } else {
+                const uint32_t w[4] = {y.x, y.y, y.z, y.w};
+                uint16_t* e = reinterpret_cast<uint16_t*>(row);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) e[2 * i] = uint16_t(w[i]), e[2 * i + 1] = uint16_t(w[i] >> 16);
-        }
-    });
+                for (int i = 0; i < 4; ++i) e[2 * i] = uint16_t(w[i]), e[2 * i + 1] = uint16_t(w[i] >> 16);
+            }
+        });
 }
 
-template <bool BF16, bool VEC>
-__global__ void __launch_bounds__(kWarps * 32)
+template <bool BF16, bool VEC, int kFlight>
+__global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm)
     load_kernel(const Rows rows, const Cache cache, const int32_t* __restrict__ slots, int32_t n, int32_t tokens) {
-    __shared__ int32_t s_slot[kMaxTokens];
+    __shared__ int64_t s_rec[kMaxTokens];
     const int64_t t0 = int64_t(blockIdx.x) * tokens;
     const int count = int(min(int64_t(tokens), n - t0));
-    if (threadIdx.x < count) {
-        const int32_t s = slots[t0 + threadIdx.x];
-        s_slot[threadIdx.x] = s >= 0 && s < cache.num_slots ? s : kZero;
+    if (threadIdx.x < kMaxTokens) {
+        int64_t rec = kSkip;
+        if (threadIdx.x < count) {
+            const int32_t s = slots[t0 + threadIdx.x];
+            rec = s >= 0 && s < cache.num_slots ? record_of(cache, s) : kZero;
+        }
+        s_rec[threadIdx.x] = rec;
     }
     __syncthreads();
-    read_rows<BF16, VEC>(rows, cache, s_slot, t0, count);
+    read_rows<BF16, VEC, kFlight>(rows, cache, s_rec, t0, count);
 }
 
-template <bool BF16, bool VEC>
-__global__ void __launch_bounds__(kWarps * 32)
+template <bool BF16, bool VEC, int kFlight>
+__global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm)
     gather_kernel(const Rows rows, const Cache cache, const int32_t* __restrict__ cu, const int32_t* __restrict__ tables,
                   int64_t bt_stride, int32_t bt_width, int32_t num_seqs, int32_t n, int32_t tokens) {
-    __shared__ int32_t s_slot[kMaxTokens];
+    __shared__ int64_t s_rec[kMaxTokens];
     const int64_t t0 = int64_t(blockIdx.x) * tokens;
     const int count = int(min(int64_t(tokens), n - t0));
-    if (threadIdx.x < count) {
+    if (threadIdx.x < kMaxTokens) {
         const int32_t t = int32_t(t0) + threadIdx.x;
-        int32_t slot = kSkip;
-        if (t >= cu[0] && t < cu[num_seqs]) {  // else: a row of no sequence
-            int lo = 0, hi = num_seqs;         // the last sequence that starts at or before t
+        int64_t rec = kSkip;
+        if (threadIdx.x < count && t >= cu[0] && t < cu[num_seqs]) {  // else: a row of no sequence
+            int lo = 0, hi = num_seqs;                               // the last sequence that starts at or before t
             while (hi - lo > 1) {
                 const int mid = (lo + hi) >> 1;
                 if (cu[mid] <= t) lo = mid; else hi = mid;
             }
             const uint32_t pos = uint32_t(t - cu[lo]), page = pos / uint32_t(cache.block_size);
-            slot = kZero;
+            rec = kZero;
             if (page < uint32_t(bt_width)) {
                 const int32_t blk = tables[lo * bt_stride + page];
                 if (blk >= 0 && int64_t(blk) * cache.block_size < cache.num_slots)
-                    slot = blk * cache.block_size + int32_t(pos - page * cache.block_size);
+                    rec = record_of(cache, blk * cache.block_size + int32_t(pos - page * cache.block_size));
             }
         }
-        s_slot[threadIdx.x] = slot;
+        s_rec[threadIdx.x] = rec;
     }
     __syncthreads();
-    read_rows<BF16, VEC>(rows, cache, s_slot, t0, count);
+    read_rows<BF16, VEC, kFlight>(rows, cache, s_rec, t0, count);
 }
 
-// Tokens per block: at least two blocks per SM while there are tokens to spare (a small call is
-// latency, spread it), at most kMaxTokens (a large one looks its slots up in bulk).
-int tokens_per_block(int32_t n) {
-    const int64_t blocks = 4 * int64_t(device_sm_count());
-    int t = 2;
-    while (t < kMaxTokens && n > blocks * t) t *= 2;
-    return t;
+// Launch shape.  Up to two tokens per resident block: latency, a pair of tokens per block and a row per
+// warp (8 tokens x 8 heads, store and load in a graph: 3.6 us against 5.4 with four pairs in flight).
+// More: whole waves of resident blocks, each of at most kMaxTokens tokens and four pairs per warp in
+// flight.  16,384 tokens x 8 heads, store and load: 40.0 us with whole waves of up to 24 tokens, 40.8
+// with powers of two up to 32; gather of 68.6k tokens: 55.8 against 56.9 us; 6 resident blocks of 40
+// registers lose 2 us on both and win 8 us of 114 on four sequences of 26k.
+struct Shape {
+    int tokens;
+    dim3 grid;
+    bool small;
+};
+
+Shape shape_of(int32_t n, int32_t hkv) {
+    const int64_t blocks = int64_t(kBlocksPerSm) * device_sm_count();
+    Shape s;
+    s.small = n <= 2 * blocks;
+    const int64_t waves = (n + kMaxTokens * blocks - 1) / (kMaxTokens * blocks);
+    s.tokens = s.small ? 2 : int((n + waves * blocks - 1) / (waves * blocks) + 1) & ~1;
+    s.grid = dim3((unsigned(n) + s.tokens - 1) / s.tokens, s.small ? (2 * hkv + kWarps - 1) / kWarps : 1);
+    return s;
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -179,7 +211,7 @@ int32_t check_common(const char* what, const void* k_rows, int64_t k_stride, con
                      const void* k_cache, const void* v_cache, int32_t num_tokens, int32_t num_kv_heads,
                      int32_t head_dim, int32_t num_blocks, int32_t block_size, int32_t dtype) {
     B200_REQUIRE(k_rows && v_rows && k_cache && v_cache, "%s: null pointer", what);
-    B200_REQUIRE(num_kv_heads > 0 && num_kv_heads <= 32768, "%s: num_kv_heads %d", what, num_kv_heads);
+    B200_REQUIRE(num_kv_heads > 0 && num_kv_heads <= 65535, "%s: num_kv_heads %d", what, num_kv_heads);
     if (head_dim != kD) return fail(B200_ERR_UNSUPPORTED, "%s: head_dim %d (only 128)", what, head_dim);
     if (dtype != B200_BF16 && dtype != B200_F16)
         return fail(B200_ERR_UNSUPPORTED, "%s: dtype %d (bf16 or fp16 only)", what, dtype);
@@ -198,18 +230,22 @@ bool vector_rows(const Rows& r) {
     return aligned16(r.k) && aligned16(r.v) && r.k_stride % 16 == 0 && r.v_stride % 16 == 0;
 }
 
-// Launches KERNEL<BF16, VEC> for the call's type and alignment.
-#define B200_Q4_LAUNCH(KERNEL, grid, stream, ...)                                                     \
-    do {                                                                                              \
-        const bool vec_ = vector_rows(rows);                                                          \
-        if (dtype == B200_BF16) {                                                                     \
-            if (vec_) KERNEL<true, true><<<grid, kWarps * 32, 0, stream>>>(__VA_ARGS__);              \
-            else KERNEL<true, false><<<grid, kWarps * 32, 0, stream>>>(__VA_ARGS__);                  \
-        } else {                                                                                      \
-            if (vec_) KERNEL<false, true><<<grid, kWarps * 32, 0, stream>>>(__VA_ARGS__);             \
-            else KERNEL<false, false><<<grid, kWarps * 32, 0, stream>>>(__VA_ARGS__);                 \
-        }                                                                                             \
-        B200_CUDA_TRY(cudaGetLastError());                                                            \
+// Launches KERNEL for the call's type, alignment and shape.
+#define B200_Q4_CASE(KERNEL, BF16, VEC, ...)                                                  \
+    do {                                                                                      \
+        if (shape.small) KERNEL<BF16, VEC, 1><<<shape.grid, kWarps * 32, 0, st>>>(__VA_ARGS__); \
+        else KERNEL<BF16, VEC, 4><<<shape.grid, kWarps * 32, 0, st>>>(__VA_ARGS__);           \
+    } while (0)
+#define B200_Q4_LAUNCH(KERNEL, n, ...)                                           \
+    do {                                                                         \
+        const Shape shape = shape_of(n, num_kv_heads);                           \
+        cudaStream_t st = static_cast<cudaStream_t>(stream);                     \
+        const bool vec = vector_rows(rows);                                      \
+        if (dtype == B200_BF16 && vec) B200_Q4_CASE(KERNEL, true, true, __VA_ARGS__, shape.tokens);  \
+        else if (dtype == B200_BF16) B200_Q4_CASE(KERNEL, true, false, __VA_ARGS__, shape.tokens);   \
+        else if (vec) B200_Q4_CASE(KERNEL, false, true, __VA_ARGS__, shape.tokens);                  \
+        else B200_Q4_CASE(KERNEL, false, false, __VA_ARGS__, shape.tokens);                          \
+        B200_CUDA_TRY(cudaGetLastError());                                       \
     } while (0)
 
 }  // namespace
@@ -233,9 +269,7 @@ extern "C" int32_t b200_store_kvcache_q4(const void* key, int64_t key_stride, co
                     key_stride * 2, value_stride * 2};
     const Cache cache{static_cast<char*>(k_cache), static_cast<char*>(v_cache), num_kv_heads, block_size,
                       int64_t(num_blocks) * block_size};
-    const int tokens = tokens_per_block(num_tokens);
-    const dim3 grid((unsigned(num_tokens) + tokens - 1) / tokens);
-    B200_Q4_LAUNCH(store_kernel, grid, static_cast<cudaStream_t>(stream), rows, cache, slot_mapping, num_tokens, tokens);
+    B200_Q4_LAUNCH(store_kernel, num_tokens, rows, cache, slot_mapping, num_tokens);
     return B200_OK;
 }
 
@@ -255,9 +289,7 @@ extern "C" int32_t b200_load_kvcache_q4(void* key, int64_t key_stride, void* val
     const Rows rows{static_cast<char*>(key), static_cast<char*>(value), key_stride * 2, value_stride * 2};
     const Cache cache{static_cast<char*>(const_cast<void*>(k_cache)), static_cast<char*>(const_cast<void*>(v_cache)),
                       num_kv_heads, block_size, int64_t(num_blocks) * block_size};
-    const int tokens = tokens_per_block(num_tokens);
-    const dim3 grid((unsigned(num_tokens) + tokens - 1) / tokens);
-    B200_Q4_LAUNCH(load_kernel, grid, static_cast<cudaStream_t>(stream), rows, cache, slot_mapping, num_tokens, tokens);
+    B200_Q4_LAUNCH(load_kernel, num_tokens, rows, cache, slot_mapping, num_tokens);
     return B200_OK;
 }
 
@@ -281,9 +313,7 @@ extern "C" int32_t b200_gather_kvcache_q4(void* key, int64_t key_stride, void* v
     const Rows rows{static_cast<char*>(key), static_cast<char*>(value), key_stride * 2, value_stride * 2};
     const Cache cache{static_cast<char*>(const_cast<void*>(k_cache)), static_cast<char*>(const_cast<void*>(v_cache)),
                       num_kv_heads, block_size, int64_t(num_blocks) * block_size};
-    const int tokens = tokens_per_block(total_tokens);
-    const dim3 grid((unsigned(total_tokens) + tokens - 1) / tokens);
-    B200_Q4_LAUNCH(gather_kernel, grid, static_cast<cudaStream_t>(stream), rows, cache, cu_seqlens, block_tables,
-                   block_table_stride, block_table_width, num_seqs, total_tokens, tokens);
+    B200_Q4_LAUNCH(gather_kernel, total_tokens, rows, cache, cu_seqlens, block_tables, block_table_stride,
+                   block_table_width, num_seqs, total_tokens);
     return B200_OK;
 }

@@ -59,10 +59,12 @@ __device__ __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b) {
 //   m = min x, s = (max x - m) / 15 rounded to the model's type (0 below 2^-100),
 //   code = min(15, rint((x - m) / s)), ties to even; a group whose max - min is not finite
 //   gets s = m = NaN and codes 0.
-// The codes are those of a correctly rounded quotient: with y = 1/s correctly rounded and q0
-// the rounded product (x - m) y, q = q0 + ((x - m) - q0 s) y in two fused operations is the
-// correctly rounded quotient (Markstein 1990; s has at most 11 significant bits and at least
-// 2^-100, so no step under- or overflows), two instructions per pair instead of a division.
+// The codes are those of the correctly rounded quotient (x - m) / s, without a division (after
+// Markstein 1990): with y ~ 1/s to 2^-23 and q0 the rounded product (x - m) y, within two units of
+// the quotient, the residual (x - m) - q0 s is exact in one fused operation, and q0 + residual * y is
+// the quotient to 2^-22 units before its rounding.  No quotient of a 24-bit by an 11-bit number is
+// that near the middle between two floats, so the rounding is the quotient's own.  The same
+// steps give the span's fifteenth.  (s is 0 or at least 2^-100, so nothing under- or overflows.)
 template <bool BF16>
 __device__ __forceinline__ uint32_t quantise8(const uint32_t (&x)[4], uint32_t& params) {
     const uint32_t mn = min2_nan<BF16>(min2_nan<BF16>(x[0], x[1]), min2_nan<BF16>(x[2], x[3]));
@@ -73,13 +75,16 @@ __device__ __forceinline__ uint32_t quantise8(const uint32_t (&x)[4], uint32_t& 
     r = min2_nan<BF16>(r, __shfl_xor_sync(0xffffffffu, r, 2));
     const float lo = lo_f<BF16>(r), span = -hi_f<BF16>(r) - lo;
     const bool finite = span <= FLT_MAX;
-    uint32_t sbits = to_bits16<BF16>(__fdiv_rn(span, 15.f));
-    float s = lo_f<BF16>(sbits);
+    constexpr float kFifteenth = 1.f / 15.f;
+    const float f0 = span * kFifteenth;
+    uint32_t sbits = to_bits16<BF16>(fmaf(fmaf(-f0, 15.f, span), kFifteenth, f0));
+    float s = lo_f<BF16>(sbits), inv;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
     if (s < kMinScale) {
         s = 0.f;
+        inv = 0.f;
         sbits = 0;
     }
-    const float inv = s > 0.f ? __frcp_rn(s) : 0.f;
     params = finite ? (sbits | (r << 16)) : 0x7fff7fffu;  // the all-ones pattern is NaN in both types
     uint32_t even = 0, odd = 0;
 #pragma unroll
@@ -88,8 +93,10 @@ __device__ __forceinline__ uint32_t quantise8(const uint32_t (&x)[4], uint32_t& 
         const float2 q0 = fmul2(d, make_float2(inv, inv));
         const float2 e = ffma2(q0, make_float2(-s, -s), d);
         float2 q = ffma2(e, make_float2(inv, inv), q0);
-        q.x = fminf(q.x, 15.f);
-        q.y = fminf(q.y, 15.f);
+        if constexpr (!BF16) {  // fp16 scales may be subnormal, off by a third; a bf16 one leaves q below 15.1
+            q.x = fminf(q.x, 15.f);
+            q.y = fminf(q.y, 15.f);
+        }
         // rint by the magic constant 1.5 * 2^23: the code lands in the low mantissa bits.  Shifting
         // moves the constant's own bits (22 and up) past bit 15, which is all that is kept.
         const float2 t = fadd2(q, make_float2(12582912.f, 12582912.f));
@@ -104,14 +111,17 @@ __device__ __forceinline__ uint32_t quantise8(const uint32_t (&x)[4], uint32_t& 
 template <bool BF16>
 __device__ __forceinline__ uint4 dequantise8(uint32_t word, uint32_t params) {
     const float s = lo_f<BF16>(params), m = hi_f<BF16>(params);
+    const uint32_t odd = word >> 16;
     uint32_t y[4];
+    float si = s;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        // 2^23 + code is exact in fp32, and so is s * code: one rounding in the sum, one to 16 bits.
-        const float2 c = fsub2(make_float2(__uint_as_float(0x4b000000u | ((word >> (4 * i)) & 15u)),
-                                           __uint_as_float(0x4b000000u | ((word >> (16 + 4 * i)) & 15u))),
+    for (int i = 0; i < 4; ++i, si *= 0.0625f) {
+        // 2^23 + 16^i code is exact in fp32, and so are s / 16^i and the product: one rounding in the
+        // sum, one to 16 bits.
+        const float2 c = fsub2(make_float2(__uint_as_float(0x4b000000u | (word & (15u << (4 * i)))),
+                                           __uint_as_float(0x4b000000u | (odd & (15u << (4 * i))))),
                                make_float2(8388608.f, 8388608.f));
-        const float2 v = ffma2(c, make_float2(s, s), make_float2(m, m));
+        const float2 v = ffma2(c, make_float2(si, si), make_float2(m, m));
         y[i] = pack2<BF16>(v.x, v.y);
     }
     return make_uint4(y[0], y[1], y[2], y[3]);
