@@ -23,11 +23,12 @@ import threading
 import torch
 
 from ._native import check, lib
-from .ops import _DTYPES, _require_cuda, _stream
+from .ops import _DTYPES
 
 HEAD_DIM = 128
 RECORD_BYTES = 80
 _CONTROL_BYTES = 16384  # covers the control words and counters at the start of an attention workspace
+_raw_stream = torch._C._cuda_getCurrentRawStream  # the handle that torch.cuda.current_stream wraps
 
 
 def q4_cache_shape(num_blocks: int, block_size: int, num_kv_heads: int, head_dim: int = HEAD_DIM) -> tuple:
@@ -37,7 +38,37 @@ def q4_cache_shape(num_blocks: int, block_size: int, num_kv_heads: int, head_dim
     return (num_blocks, num_kv_heads, block_size, RECORD_BYTES)
 
 
-def _check_caches(k_cache, v_cache, num_kv_heads):
+# The checks.  A decode step makes two of these calls per layer, and for small batches the host is what
+# bounds them: each op asks once whether everything holds and only looks for the reason if it does not.
+def _cache_ok(k_cache, v_cache, num_kv_heads):
+    shape = k_cache.shape
+    return (k_cache.dtype == torch.uint8 == v_cache.dtype and len(shape) == 4 and shape[3] == RECORD_BYTES
+            and shape[1] == num_kv_heads and v_cache.shape == shape and k_cache.is_contiguous()
+            and v_cache.is_contiguous())
+
+
+def _rows_ok(key, value):
+    shape, ks, vs = key.shape, key.stride(), value.stride()
+    return (len(shape) == 3 and shape[2] == HEAD_DIM and value.shape == shape and key.dtype in _DTYPES
+            and value.dtype == key.dtype and ks[2] == 1 == vs[2]
+            and (shape[1] == 1 or ks[1] == HEAD_DIM == vs[1]))
+
+
+def _same_device(index, *tensors):
+    for t in tensors:
+        if t.get_device() != index:
+            return False
+    return index >= 0
+
+
+def _refuse_type(dtype, head_dim):
+    if head_dim != HEAD_DIM:
+        raise NotImplementedError(f"4-bit KV cache: head_dim {head_dim} (only {HEAD_DIM})")
+    if dtype not in _DTYPES:
+        raise NotImplementedError(f"4-bit KV cache: dtype {dtype} (bf16 or fp16 only)")
+
+
+def _explain_cache(k_cache, v_cache, num_kv_heads):
     assert k_cache.dtype == v_cache.dtype == torch.uint8, "4-bit KV caches are uint8 tensors"
     assert k_cache.dim() == 4 and k_cache.shape == v_cache.shape and k_cache.size(3) == RECORD_BYTES, \
         "4-bit KV caches are [num_blocks, num_kv_heads, block_size, 80]"
@@ -45,22 +76,30 @@ def _check_caches(k_cache, v_cache, num_kv_heads):
     assert k_cache.size(1) == num_kv_heads, f"cache of {k_cache.size(1)} kv heads, rows of {num_kv_heads}"
 
 
-def _check_slots(slot_mapping, n):
-    assert slot_mapping.dtype == torch.int32 and slot_mapping.is_contiguous(), "slot_mapping must be contiguous int32"
-    assert slot_mapping.numel() == n
+def _explain_rows(key, value):
+    assert key.dim() == 3 and value.shape == key.shape, "key and value must be [N, Hkv, 128] of one shape"
+    _refuse_type(key.dtype, key.size(2))
+    assert value.dtype == key.dtype, "key/value dtypes differ"
+    raise AssertionError("rows must hold their heads contiguously")
 
 
-def _check_rows(key, value):
-    N, H, D = key.shape
-    assert value.shape == key.shape, "key and value shapes differ"
-    if D != HEAD_DIM:
-        raise NotImplementedError(f"4-bit KV cache: head_dim {D} (only {HEAD_DIM})")
-    assert key.dtype == value.dtype, "key/value dtypes differ"
-    if key.dtype not in _DTYPES:
-        raise NotImplementedError(f"4-bit KV cache: dtype {key.dtype} (bf16 or fp16 only)")
-    for t in (key, value):
-        assert t.stride(-1) == 1 and (H == 1 or t.stride(1) == D), "rows must hold their heads contiguously"
-    return N, H
+def _explain_ints(what, t):
+    raise AssertionError(f"{what} must be int32 and contiguous, of the call's size, not {t.dtype} {tuple(t.shape)}")
+
+
+def _explain_devices(*tensors):
+    raise AssertionError(f"4-bit KV cache ops take CUDA tensors of one device, not {[str(t.device) for t in tensors]}")
+
+
+def _call(name, index, fn, *args):
+    """fn(*args, stream) with device `index` current and its current stream; raises for a status."""
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc:
+        check(rc, name)
 
 
 def _token_stride(t):
@@ -75,27 +114,33 @@ def store_kvcache_q4(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tens
     Slots of -1 (padding) or outside the cache are skipped; the others must be
     unique within one call (as for `store_kvcache`).
     """
-    N, H = _check_rows(key, value)
-    _check_caches(k_cache, v_cache, H)
-    _check_slots(slot_mapping, N)
-    _require_cuda(key, value, k_cache, v_cache, slot_mapping)
-    with torch.cuda.device(key.device):
-        rc = lib().b200_store_kvcache_q4(key.data_ptr(), _token_stride(key), value.data_ptr(), _token_stride(value),
-                                         k_cache.data_ptr(), v_cache.data_ptr(), slot_mapping.data_ptr(), N, H,
-                                         HEAD_DIM, k_cache.size(0), k_cache.size(2), _DTYPES[key.dtype], _stream(key))
-    check(rc, "store_kvcache_q4")
+    if not _rows_ok(key, value):
+        _explain_rows(key, value)
+    N, H, _ = key.shape
+    if not _cache_ok(k_cache, v_cache, H):
+        _explain_cache(k_cache, v_cache, H)
+    if slot_mapping.dtype != torch.int32 or slot_mapping.numel() != N or not slot_mapping.is_contiguous():
+        _explain_ints("slot_mapping", slot_mapping)
+    dev = key.get_device()
+    if not _same_device(dev, value, k_cache, v_cache, slot_mapping):
+        _explain_devices(key, value, k_cache, v_cache, slot_mapping)
+    NB, _, bs, _ = k_cache.shape
+    _call("store_kvcache_q4", dev, lib().b200_store_kvcache_q4, key.data_ptr(), _token_stride(key), value.data_ptr(),
+          _token_stride(value), k_cache.data_ptr(), v_cache.data_ptr(), slot_mapping.data_ptr(), N, H, HEAD_DIM, NB, bs,
+          _DTYPES[key.dtype])
 
 
 def _out_rows(out, n, k_cache, dtype):
-    if dtype not in _DTYPES:
-        raise NotImplementedError(f"4-bit KV cache: dtype {dtype} (bf16 or fp16 only)")
+    """The (key, value) rows a reader writes."""
+    H = k_cache.size(1)
     if out is None:
-        shape = (n, k_cache.size(1), HEAD_DIM)
-        return (torch.empty(shape, dtype=dtype, device=k_cache.device),
-                torch.empty(shape, dtype=dtype, device=k_cache.device))
+        _refuse_type(dtype, HEAD_DIM)
+        return k_cache.new_empty((n, H, HEAD_DIM), dtype=dtype), k_cache.new_empty((n, H, HEAD_DIM), dtype=dtype)
     key, value = out
-    _check_rows(key, value)
-    assert key.size(0) == n and key.dtype == dtype, "out rows do not match the tokens and dtype asked for"
+    if not _rows_ok(key, value):
+        _explain_rows(key, value)
+    assert key.size(0) == n and key.size(1) == H and key.dtype == dtype, \
+        "out rows do not match the tokens, kv heads and dtype asked for"
     return key, value
 
 
@@ -104,18 +149,20 @@ def load_kvcache_q4(k_cache: torch.Tensor, v_cache: torch.Tensor, slot_mapping: 
     """Read the records of slot_mapping [N] back: (key, value) rows [N, Hkv, 128] in `dtype`, the type
     the cache was written in.  Slots of -1 or outside the cache read as zeros.  `out` is an optional
     (key, value) pair to write to."""
-    _check_caches(k_cache, v_cache, k_cache.size(1))
+    H = k_cache.size(1)
+    if not _cache_ok(k_cache, v_cache, H):
+        _explain_cache(k_cache, v_cache, H)
     N = slot_mapping.numel()
-    _check_slots(slot_mapping, N)
+    if slot_mapping.dtype != torch.int32 or not slot_mapping.is_contiguous():
+        _explain_ints("slot_mapping", slot_mapping)
     key, value = _out_rows(out, N, k_cache, dtype)
-    assert key.size(1) == k_cache.size(1), "out rows and cache differ in kv heads"
-    _require_cuda(k_cache, v_cache, slot_mapping, key, value)
-    with torch.cuda.device(k_cache.device):
-        rc = lib().b200_load_kvcache_q4(key.data_ptr(), _token_stride(key), value.data_ptr(), _token_stride(value),
-                                        k_cache.data_ptr(), v_cache.data_ptr(), slot_mapping.data_ptr(), N,
-                                        k_cache.size(1), HEAD_DIM, k_cache.size(0), k_cache.size(2), _DTYPES[dtype],
-                                        _stream(k_cache))
-    check(rc, "load_kvcache_q4")
+    dev = k_cache.get_device()
+    if not _same_device(dev, v_cache, slot_mapping, key, value):
+        _explain_devices(k_cache, v_cache, slot_mapping, key, value)
+    NB, _, bs, _ = k_cache.shape
+    _call("load_kvcache_q4", dev, lib().b200_load_kvcache_q4, key.data_ptr(), _token_stride(key), value.data_ptr(),
+          _token_stride(value), k_cache.data_ptr(), v_cache.data_ptr(), slot_mapping.data_ptr(), N, H, HEAD_DIM, NB, bs,
+          _DTYPES[dtype])
     return key, value
 
 
@@ -130,23 +177,24 @@ def gather_kvcache_q4(k_cache: torch.Tensor, v_cache: torch.Tensor, cu_seqlens: 
     behind the last sequence are left as they were); None reads cu_seqlens[-1] on the host,
     which synchronises.  Tokens of a page outside the cache read as zeros.
     """
-    _check_caches(k_cache, v_cache, k_cache.size(1))
-    assert cu_seqlens.dtype == torch.int32 and cu_seqlens.is_contiguous() and cu_seqlens.numel() >= 1
+    H = k_cache.size(1)
+    if not _cache_ok(k_cache, v_cache, H):
+        _explain_cache(k_cache, v_cache, H)
     S = cu_seqlens.numel() - 1
-    assert block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.stride(1) == 1
-    assert block_table.size(0) >= S, "block_table has fewer rows than sequences"
+    if cu_seqlens.dtype != torch.int32 or S < 0 or not cu_seqlens.is_contiguous():
+        _explain_ints("cu_seqlens", cu_seqlens)
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.stride(1) != 1 or block_table.size(0) < S:
+        _explain_ints("block_table (a row per sequence)", block_table)
     n = int(cu_seqlens[-1]) if total_tokens is None else int(total_tokens)
     assert n >= 0, f"total_tokens {n} < 0"
     key, value = _out_rows(out, n, k_cache, dtype)
-    assert key.size(1) == k_cache.size(1), "out rows and cache differ in kv heads"
-    _require_cuda(k_cache, v_cache, cu_seqlens, block_table, key, value)
-    with torch.cuda.device(k_cache.device):
-        rc = lib().b200_gather_kvcache_q4(key.data_ptr(), _token_stride(key), value.data_ptr(), _token_stride(value),
-                                          k_cache.data_ptr(), v_cache.data_ptr(), cu_seqlens.data_ptr(),
-                                          block_table.data_ptr(), block_table.stride(0), block_table.size(1), S, n,
-                                          k_cache.size(1), HEAD_DIM, k_cache.size(0), k_cache.size(2), _DTYPES[dtype],
-                                          _stream(k_cache))
-    check(rc, "gather_kvcache_q4")
+    dev = k_cache.get_device()
+    if not _same_device(dev, v_cache, cu_seqlens, block_table, key, value):
+        _explain_devices(k_cache, v_cache, cu_seqlens, block_table, key, value)
+    NB, _, bs, _ = k_cache.shape
+    _call("gather_kvcache_q4", dev, lib().b200_gather_kvcache_q4, key.data_ptr(), _token_stride(key), value.data_ptr(),
+          _token_stride(value), k_cache.data_ptr(), v_cache.data_ptr(), cu_seqlens.data_ptr(), block_table.data_ptr(),
+          block_table.stride(0), block_table.size(1), S, n, H, HEAD_DIM, NB, bs, _DTYPES[dtype])
     return key, value
 
 
@@ -164,20 +212,45 @@ def q4_workspace_size(query_len: int, group: int) -> int:
 def q4_workspace(device: torch.device, query_len: int, group: int) -> torch.Tensor:
     """The split-K workspace of a call on the current stream, its control words and counters zero.
 
-    Eager calls keep one per (device, stream), grown on demand: calls of one stream run one after
-    another and leave it re-armed.  A call that is being captured gets its own from the graph's
+    Eager calls keep one per (device, stream), for up to 16 query rows: calls of one stream run one
+    after another and leave it re-armed.  A call that is being captured gets its own from the graph's
     memory pool, zeroed by the graph itself, so that graphs replayed at the same time share nothing."""
-    need = q4_workspace_size(query_len, group)
+    index = device.index if device.index is not None else torch.cuda.current_device()
+    with torch.cuda.device(index):
+        return _workspace(index, query_len * group)
+
+
+def _workspace(index, rows):
     if torch.cuda.is_current_stream_capturing():
-        ws = torch.empty(need, dtype=torch.uint8, device=device)
+        ws = torch.empty(q4_workspace_size(rows, 1), dtype=torch.uint8, device=torch.device("cuda", index))
         ws[:_CONTROL_BYTES].zero_()
         return ws
-    key = (device.index, torch.cuda.current_stream(device).cuda_stream)
-    with _ws_lock:
-        ws = _workspaces.get(key)
-        if ws is None or ws.numel() < need:
-            ws = _workspaces[key] = torch.zeros(need, dtype=torch.uint8, device=device)
+    key = (index, _raw_stream(index))
+    ws = _workspaces.get(key)
+    if ws is None:
+        with _ws_lock:
+            ws = _workspaces.get(key)
+            if ws is None:
+                ws = torch.zeros(q4_workspace_size(16, 1), dtype=torch.uint8, device=torch.device("cuda", index))
+                _workspaces[key] = ws
     return ws
+
+
+def _explain_attention(q, k_cache, v_cache, cache_seqlens, block_table, causal, out):
+    B, Lq, Hq, D = q.shape
+    _refuse_type(q.dtype, D)
+    Hkv = k_cache.size(1)
+    _explain_cache(k_cache, v_cache, Hkv)
+    assert Hkv > 0 and Hq % Hkv == 0, f"num_heads {Hq} not a multiple of num_kv_heads {Hkv}"
+    assert q.stride(-1) == 1 and (Hq == 1 or q.stride(-2) == D), "q heads must be contiguous"
+    assert Lq == 1 or B <= 1 or q.stride(0) == Lq * q.stride(1), "q rows of one sequence must be evenly strided"
+    assert cache_seqlens.dtype == torch.int32 and cache_seqlens.is_contiguous() and cache_seqlens.numel() == B, \
+        "cache_seqlens must be contiguous int32, one per sequence"
+    assert block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.stride(1) == 1, \
+        "block_table must be int32 [B, W] with contiguous rows"
+    assert block_table.size(0) >= B, "block_table has fewer rows than q"
+    assert out.shape == q.shape and out.is_contiguous() and out.dtype == q.dtype, "out must be contiguous and like q"
+    _explain_devices(q, k_cache, v_cache, cache_seqlens, block_table, out)
 
 
 def flash_attn_with_kvcache_q4(q, k_cache, v_cache, cache_seqlens=None, block_table=None, softmax_scale=None,
@@ -195,33 +268,29 @@ def flash_attn_with_kvcache_q4(q, k_cache, v_cache, cache_seqlens=None, block_ta
     B, Lq, Hq, D = q.shape
     if not causal and Lq > 1:
         raise NotImplementedError("non-causal multi-query paged attention")
-    if D != HEAD_DIM:
-        raise NotImplementedError(f"4-bit KV cache: head_dim {D} (only {HEAD_DIM})")
-    if q.dtype not in _DTYPES:
-        raise NotImplementedError(f"4-bit KV cache: dtype {q.dtype} (bf16 or fp16 only)")
-    Hkv = k_cache.size(1)
-    _check_caches(k_cache, v_cache, Hkv)
-    assert Hkv > 0 and Hq % Hkv == 0, f"num_heads {Hq} not a multiple of num_kv_heads {Hkv}"
-    assert q.stride(-1) == 1 and (Hq == 1 or q.stride(-2) == D), "q heads must be contiguous"
-    if Lq == 1:
-        q_tok = q.stride(0) if B > 1 else Hq * D
-    else:
-        assert B <= 1 or q.stride(0) == Lq * q.stride(1), "q rows of one sequence must be evenly strided"
-        q_tok = q.stride(1)
-    assert cache_seqlens.dtype == torch.int32 and cache_seqlens.is_contiguous() and cache_seqlens.numel() == B
-    assert block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.stride(1) == 1
-    assert block_table.size(0) >= B, "block_table has fewer rows than q"
+    NB, Hkv, bs, _ = k_cache.shape
     if out is None:
-        out = torch.empty((B, Lq, Hq, D), dtype=q.dtype, device=q.device)
-    else:
-        assert out.shape == (B, Lq, Hq, D) and out.is_contiguous() and out.dtype == q.dtype
-    _require_cuda(q, k_cache, v_cache, cache_seqlens, block_table, out)
-    scale = D ** -0.5 if softmax_scale is None else softmax_scale
-    with torch.cuda.device(q.device):
-        ws = q4_workspace(q.device, Lq, Hq // Hkv) if workspace is None else workspace
-        rc = lib().b200_paged_attention_q4(out.data_ptr(), q.data_ptr(), q_tok, k_cache.data_ptr(), v_cache.data_ptr(),
-                                           k_cache.size(0), k_cache.size(2), block_table.data_ptr(),
-                                           block_table.stride(0), block_table.size(1), cache_seqlens.data_ptr(), B, Lq, Hq, Hkv, D,
-                                           float(scale), _DTYPES[q.dtype], ws.data_ptr(), ws.numel(), _stream(q))
-    check(rc, "flash_attn_with_kvcache_q4")
+        out = q.new_empty((B, Lq, Hq, D))
+    qs = q.stride()
+    q_tok = (qs[0] if B > 1 else Hq * D) if Lq == 1 else qs[1]
+    dev = q.get_device()
+    if not (D == HEAD_DIM and q.dtype in _DTYPES and _cache_ok(k_cache, v_cache, Hkv) and Hkv > 0 and Hq % Hkv == 0
+            and qs[3] == 1 and (Hq == 1 or qs[2] == D) and (Lq == 1 or B <= 1 or qs[0] == Lq * qs[1])
+            and cache_seqlens.dtype == torch.int32 and cache_seqlens.numel() == B and cache_seqlens.is_contiguous()
+            and block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.stride(1) == 1
+            and block_table.size(0) >= B and out.shape == q.shape and out.is_contiguous() and out.dtype == q.dtype
+            and _same_device(dev, k_cache, v_cache, cache_seqlens, block_table, out)):
+        _explain_attention(q, k_cache, v_cache, cache_seqlens, block_table, causal, out)
+    if workspace is None:
+        rows = min(Lq * (Hq // Hkv), 16)
+        if torch._C._cuda_getDevice() == dev:
+            workspace = _workspace(dev, rows)
+        else:
+            with torch.cuda.device(dev):
+                workspace = _workspace(dev, rows)
+    _call("flash_attn_with_kvcache_q4", dev, lib().b200_paged_attention_q4, out.data_ptr(), q.data_ptr(), q_tok,
+          k_cache.data_ptr(), v_cache.data_ptr(), NB, bs, block_table.data_ptr(), block_table.stride(0),
+          block_table.size(1), cache_seqlens.data_ptr(), B, Lq, Hq, Hkv, D,
+          D ** -0.5 if softmax_scale is None else float(softmax_scale), _DTYPES[q.dtype], workspace.data_ptr(),
+          workspace.numel())
     return out
