@@ -57,11 +57,11 @@ using q4::lo_f;
 
 constexpr int kTile = 128;  // tokens per stage
 constexpr int kWarps = 4;   // consumer warps
+constexpr int kWarpTokens = kTile / kWarps;
+constexpr int kQBufs = 2;   // items whose query rows fit
 constexpr int kConsumers = kWarps * 32;
 constexpr int kThreads = kConsumers + 32;
-constexpr int kCtas = 3;    // per SM
-constexpr int kStages = 3;
-constexpr int kQBufs = 2;
+constexpr int kStages = 2;
 constexpr int kKvBytes = kTile * kRecord;  // keys (or values) of one stage
 constexpr int kStageBytes = 2 * kKvBytes;
 constexpr int kMaxBatch = 2048;
@@ -69,20 +69,6 @@ constexpr int kPairCost = 2;  // what a (sequence, kv head) pair costs beside it
 constexpr float kLazyMax = 8.f;  // log2 headroom before a row's running maximum is raised
 constexpr float kNone = -1e30f;  // reference of a row that has met no token
 constexpr int kExpMax = 60;      // bound of |E| and of the query rows' exponents
-// Least E.  fp16 operands hold p * 2^-E itself: below 2^15 with p <= 2^kLazyMax.
-template <bool BF16>
-constexpr int kExpMin = BF16 ? -kExpMax : -7;
-
-// All CTAs of the grid are resident (three per SM).
-int grid_ctas() { return device_sm_count() * kCtas; }
-
-// Workspace: control words ([2] error word), counters of the CTAs' last items (one per consumer
-// warp), two partial results per CTA and, once per consumer warp, their log-sum-exps.
-constexpr size_t kCtrlBytes = 256;
-size_t fixed_bytes(int ctas) { return kCtrlBytes + ((size_t(ctas) * kWarps * 4 + 255) & ~size_t(255)); }
-size_t workspace_bytes(int rows, int ctas) {
-    return (fixed_bytes(ctas) + size_t(2) * ctas * rows * (kD + kWarps) * 4 + 255) & ~size_t(255);
-}
 
 struct Params {
     const uint16_t* q;
@@ -112,34 +98,46 @@ struct Header {
 };
 enum : int32_t { kFirst = 1, kLast = 2, kNoPage = 4, kQBuf = 8 };
 
-// ROWS16: 9 to 16 query rows.
-template <bool ROWS16>
+// NT: groups of 8 query rows (2 for 9 to 16 rows).
+template <int NT>
 struct Cfg {
-    static constexpr int kHalves = ROWS16 ? 2 : 1;              // groups of 8 query rows
-    static constexpr int kSlices = kWarps / kHalves;            // warps that share a group of rows
-    static constexpr int kWarpTokens = kTile / kSlices;
-    static constexpr int kPassRows = 4 / kHalves;               // rows of a group combined at a time
+    // Per SM.  Up to 8 rows take 128 registers a thread, which 15 warps leave; up to 16 take 168.
+    static constexpr int kCtas = NT == 1 ? 3 : 2;
+    static constexpr int kPassRows = NT == 1 ? 4 : 16;  // rows combined at a time (what shared memory leaves)
 };
+
+// All CTAs of the grid are resident.
+int grid_ctas(int rows) { return device_sm_count() * (rows > 8 ? Cfg<2>::kCtas : Cfg<1>::kCtas); }
+
+// Workspace: control words ([2] error word), counters of the CTAs' last items (one per consumer
+// warp), two partial results per CTA and, once per consumer warp, their log-sum-exps.
+constexpr size_t kCtrlBytes = 256;
+size_t fixed_bytes(int ctas) { return kCtrlBytes + ((size_t(ctas) * kWarps * 4 + 255) & ~size_t(255)); }
+size_t workspace_bytes(int rows) {
+    const int ctas = grid_ctas(rows);
+    return (fixed_bytes(ctas) + size_t(2) * ctas * rows * (kD + kWarps) * 4 + 255) & ~size_t(255);
+}
 
 constexpr int kRowPad = kD + 1;  // floats: the lanes of a fragment write 32 different banks
 
-template <bool ROWS16>
+template <int NT>
 struct Smem {
     alignas(128) uint8_t stages[kStages][kStageBytes];
-    uint8_t qbuf[kQBufs][8 * Cfg<ROWS16>::kHalves * kD * 2];
-    float co[kWarps][Cfg<ROWS16>::kPassRows][kRowPad];
-    float cm[kWarps][Cfg<ROWS16>::kPassRows];
-    float cl[kWarps][Cfg<ROWS16>::kPassRows];
-    alignas(16) uint32_t ones[4];  // a row of ones in the model's type
+    uint8_t qbuf[kQBufs][8 * NT * kD * 2];
+    float co[kWarps][Cfg<NT>::kPassRows][kRowPad];
+    float cm[kWarps][Cfg<NT>::kPassRows];
+    float cl[kWarps][Cfg<NT>::kPassRows];
+    alignas(16) uint32_t ones[4];  // a row of fp16 ones
     Header hdr[kStages];
+    Header part[kWarps][2];        // the run's partial items, as each warp left them
     uint64_t full[kStages];
     uint64_t empty[kStages];
     uint64_t cbar;
-    int32_t off[kConsumers];  // length before each entry of ceil(batch / 128) sequences
+    int32_t off[kConsumers / 2];  // length before each entry of 2 ceil(batch / 128) sequences
     int32_t red[kWarps];
     int32_t err;
 };
-static_assert(sizeof(Smem<false>) <= 233472 / kCtas - 1024 && sizeof(Smem<true>) <= 233472 / kCtas - 1024,
+static_assert(sizeof(Smem<1>) <= 233472 / Cfg<1>::kCtas - 1024 && sizeof(Smem<2>) <= 233472 / Cfg<2>::kCtas - 1024,
               "shared memory over the SM's");
 
 __device__ __forceinline__ void bulk_load_hint(void* dst, const void* src, uint32_t bytes, uint64_t* bar,
@@ -205,6 +203,30 @@ __device__ __forceinline__ uint32_t finite2(uint32_t w) {
     return w;
 }
 
+__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+__device__ __forceinline__ uint32_t fma_f16x2(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t d;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+    return d;
+}
+
+// max(16 s, |m|) over four parameter words (NaNs apart).
+template <bool BF16>
+__device__ __forceinline__ float reach_of(const uint4& w) {
+    auto maxabs = [](uint32_t a, uint32_t b) {  // the larger magnitudes; their signs are no matter
+        uint32_t d;
+        if constexpr (BF16) asm("max.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+        else asm("max.xorsign.abs.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+        return d;
+    };
+    const uint32_t m = maxabs(maxabs(w.x, w.y), maxabs(w.z, w.w));
+    return fmaxf(fabsf(lo_f<BF16>(m)) * 16.f, fabsf(hi_f<BF16>(m)));
+}
+
 // Barrier of the consumer threads, bounded.  False, for the whole warp alike, when a lane's wait ran out.
 __device__ __forceinline__ bool consumer_wait(uint64_t* bar, uint32_t& phase, uint64_t limit_ns) {
     const bool ok = mbar_wait_spin(bar, phase, limit_ns);
@@ -223,17 +245,17 @@ __device__ __forceinline__ int64_t out_row(const Params& p, int b, int h, int r)
     return ((int64_t(b) * p.lq + j) * p.hq + h * p.group + (r - j * p.group)) * kD;
 }
 
-// Merges the chunks of a split pair for the rows [row0, row0 + n) and this warp's share of each pass
-// of kPassRows of them; called by the warp that finished the last chunk.
-template <bool BF16, bool ROWS16>
-__device__ __forceinline__ void merge_share(const Params& p, const Header& hd, int row0, int n, int warp, int lane) {
-    using C = Cfg<ROWS16>;
-    for (int r0 = 0; r0 < n; r0 += C::kPassRows) {
-        const int share = min(C::kPassRows, n - r0) * (kD / C::kSlices);
+// Merges the chunks of a split pair for this warp's share of each pass of kPassRows rows; called by the
+// warp that finished the last chunk.
+template <bool BF16, int NT>
+__device__ __forceinline__ void merge_share(const Params& p, const Header& hd, int warp, int lane) {
+    using C = Cfg<NT>;
+    for (int r0 = 0; r0 < p.rows; r0 += C::kPassRows) {
+        const int share = min(C::kPassRows, p.rows - r0) * (kD / kWarps);
         for (int i = 4 * lane; i < share; i += 128) {
-            const int e = (row0 + r0) * kD + (warp % C::kSlices) * share + i, r = e >> 7, d = e & (kD - 1);
+            const int e = r0 * kD + warp * share + i, r = e >> 7, d = e & (kD - 1);
             float m = -INFINITY, den = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-            constexpr int kFlight = 8;  // chunks whose loads are in flight
+                        constexpr int kFlight = 8;  // chunks whose loads are in flight
             for (int c0 = 0; c0 < hd.nch; c0 += kFlight) {
                 float lse[kFlight];
                 float4 x[kFlight];
@@ -273,11 +295,11 @@ __device__ __forceinline__ void merge_share(const Params& p, const Header& hd, i
     }
 }
 
-template <bool BF16, bool ROWS16>
-__global__ void __launch_bounds__(kThreads, kCtas) paged_attention_q4_kernel(const __grid_constant__ Params p) {
-    using C = Cfg<ROWS16>;
+template <bool BF16, int NT>
+__global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_kernel(const __grid_constant__ Params p) {
+    using C = Cfg<NT>;
     extern __shared__ uint8_t smem_raw[];
-    Smem<ROWS16>& sm = *reinterpret_cast<Smem<ROWS16>*>(smem_raw);
+    Smem<NT>& sm = *reinterpret_cast<Smem<NT>*>(smem_raw);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int cap = p.bt_width * p.block_size;  // tokens addressable through the block table
 
@@ -288,12 +310,12 @@ __global__ void __launch_bounds__(kThreads, kCtas) paged_attention_q4_kernel(con
         }
         mbar_init(&sm.cbar, kConsumers);
         sm.err = 0;
-        for (int i = 0; i < 4; ++i) sm.ones[i] = BF16 ? 0x3f803f80u : 0x3c003c00u;
+        for (int i = 0; i < 4; ++i) sm.ones[i] = 0x3c003c00u;
         fence_mbar_init();
     }
 
     // ---- plan: this CTA's run ------------------------------------------
-    const int run = (p.batch + kConsumers - 1) / kConsumers;  // sequences per entry of off[]
+    const int run = (p.batch + kConsumers - 1) / kConsumers;  // sequences per thread; off[] has every second
     int total;                                                // length of all pairs
     {
         int mine = 0, before = 0;
@@ -313,7 +335,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) paged_attention_q4_kernel(con
             if (w < warp) before += sm.red[w];
             total += sm.red[w];
         }
-        if (warp < kWarps) sm.off[tid] = before - mine;
+        if (warp < kWarps && !(tid & 1)) sm.off[tid >> 1] = before - mine;
         total *= p.hkv;
         __syncthreads();
     }
@@ -336,12 +358,12 @@ __global__ void __launch_bounds__(kThreads, kCtas) paged_attention_q4_kernel(con
             const uint64_t pol = l2_policy_evict_first();
             const uint32_t q_bytes = uint32_t(p.group) * kD * 2;  // one query token's rows of this kv head
             // First pair of the run: its entry of off[] by binary search, then along the entry.
-            int lo = 0, hi = kConsumers;
+            int lo = 0, hi = kConsumers / 2;
             while (hi - lo > 1) {
                 const int mid = (lo + hi) >> 1;
                 if (sm.off[mid] * p.hkv <= begin) lo = mid; else hi = mid;
             }
-            int b = lo * run, at = sm.off[lo] * p.hkv;  // `at`: where the current pair begins
+            int b = 2 * lo * run, at = sm.off[lo] * p.hkv;  // `at`: where the current pair begins
             int ctx = min(p.context_lens[b], cap), nt = tiles_of(ctx, cap);
             while (at + span_of(nt) * p.hkv <= begin) {
                 at += span_of(nt) * p.hkv;
@@ -373,7 +395,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) paged_attention_q4_kernel(con
             int stage = 0, qb = 0;
             uint32_t phase = 0;
             int fills = 0;
-            int q_fill[kQBufs] = {-kStages, -kStages};  // fill that brought the query rows of each buffer
+            int q_fill[2] = {-kStages, -kStages};  // fill that brought the query rows of each buffer
             bool ok = true;
             int first_flag = kFirst;
             while (at + t < end) {
@@ -448,9 +470,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) paged_attention_q4_kernel(con
 
     // ---------------------------------------------------------------- consumers
     const int g = lane >> 2, c = lane & 3;
-    const int row_base = 8 * (warp / C::kSlices);         // this warp's query rows
-    const int tok_warp = (warp % C::kSlices) * C::kWarpTokens;
-    const int rows = min(8, p.rows - row_base);           // of them, those that exist
+    const int tok_warp = warp * kWarpTokens;
     // Byte offsets in a sub-tile's records: the rows this lane hands to ldmatrix (token lane & 7, group
     // lane >> 3; the parameters of token lane & 15; transposed, those of token (lane & 7) + 8 (lane >> 4)
     // or a row of ones), the parameters of token g, and those this lane looks over.
@@ -460,17 +480,19 @@ __global__ void __launch_bounds__(kThreads, kCtas) paged_attention_q4_kernel(con
     const uint32_t trans_off = uint32_t((lane & 7) + (lane >> 4) * 8) * kRecord + q4::kParams;
     const uint32_t look_off = uint32_t(lane) * kRecord + q4::kParams;
     constexpr uint32_t kLo = 0x000f000fu, kHi = 0x00f000f0u;
+    if (lane < 2) sm.part[warp][lane].nch = 0;
+    __syncwarp();
     int stage = 0;
     uint32_t phase = 0, cphase = 0;
-    // Query rows 2 c + e: reference (log2), factor of the scores, limit.
-    float r_ref[2], f_row[2];
-    int lim[2];
+    // Query rows 8 nt + 2 c + e: reference (log2), factor of the scores, limit.
+    float r_ref[NT][2], f_row[NT][2];
+    int lim[NT][2];
     int lim_min = 0;
-    uint32_t qf[kGroups][2][2], qs[2];  // B operands of row g: q, and (0, sum q) of group c
+    uint32_t qf[kGroups][NT][4], qs[NT][2];  // B operands of row 8 nt + g: q (two steps of a group), (0, sum q) of group c
     // O^T fragments (16 dims x 8 rows in units of 2^-24), and the product with the parameter words:
     // its row g is sum_t p * (half-word g), rows 8.. are sum_t p.
-    float o[kGroups][2][4], om[4];
-    float y_lim = 0.f, s_lim = 0.f;  // kLazyMax - E, and the value scale that E allows
+    float o[kGroups][2][NT][4], om[NT][4];
+    float unit = 1.f, reach_lim = 0.f;  // 2^-E, and the reach of value parameters that E allows
     bool reading = false;            // the last combine's shared memory may still be read by other warps
     while (true) {
         // Exit decisions are warp-uniform (the lanes' waits can disagree at the limit).
@@ -485,63 +507,67 @@ __global__ void __launch_bounds__(kThreads, kCtas) paged_attention_q4_kernel(con
         if (__any_sync(0xffffffffu, flags & kFirst)) {
             // A sibling consumer warp that gave up will not reach the consumer barrier below.
             if (__any_sync(0xffffffffu, *reinterpret_cast<volatile int32_t*>(&sm.err) != 0)) break;
-            const uint8_t* qrow = sm.qbuf[flags & kQBuf ? 1 : 0] + (row_base + g) * kD * 2;
-            float x[kGroups][8];
-            float mx = 0.f;
 #pragma unroll
-            for (int j = 0; j < kGroups; ++j) {
-                uint4 w = make_uint4(0, 0, 0, 0);
-                if (g < rows) w = *reinterpret_cast<const uint4*>(qrow + (32 * j + 8 * c) * 2);
-                const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+            for (int nt = 0; nt < NT; ++nt) {
+                const int row = 8 * nt + g;
+                const uint8_t* qrow = sm.qbuf[flags & kQBuf ? 1 : 0] + row * kD * 2;
+                float x[kGroups][8];
+                float mx = 0.f;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    x[j][2 * i] = lo_f<BF16>(u[i]);
-                    x[j][2 * i + 1] = hi_f<BF16>(u[i]);
-                    mx = max3f(mx, fabsf(x[j][2 * i]), fabsf(x[j][2 * i + 1]));
+                for (int j = 0; j < kGroups; ++j) {
+                    uint4 w = make_uint4(0, 0, 0, 0);
+                    if (row < p.rows) w = *reinterpret_cast<const uint4*>(qrow + (32 * j + 8 * c) * 2);
+                    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        x[j][2 * i] = lo_f<BF16>(u[i]);
+                        x[j][2 * i + 1] = hi_f<BF16>(u[i]);
+                        mx = max3f(mx, fabsf(x[j][2 * i]), fabsf(x[j][2 * i + 1]));
+                    }
                 }
-            }
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            const int eq = mx > 0.f ? min(max((__float_as_int(mx) >> 23) - 127 - 3, -kExpMax), kExpMax) : 0;
-            const float sc = exp2_int(-eq);
-            float mine = 0.f;  // sum(q) of group c
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                const int eq = mx > 0.f ? min(max((__float_as_int(mx) >> 23) - 127 - 3, -kExpMax), kExpMax) : 0;
+                const float sc = exp2_int(-eq);
+                float mine = 0.f;  // sum(q) of group c
 #pragma unroll
-            for (int j = 0; j < kGroups; ++j) {
-                float sum = 0.f;
+                for (int j = 0; j < kGroups; ++j) {
+                    float sum = 0.f;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    x[j][i] *= sc;
-                    sum += x[j][i];
+                    for (int i = 0; i < 8; ++i) {
+                        x[j][i] *= sc;
+                        sum += x[j][i];
+                    }
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                    if (c == j) mine = sum;
+                    qf[j][nt][0] = pack2<false>(x[j][0], x[j][1]);
+                    qf[j][nt][1] = pack2<false>(x[j][2] * 0.0625f, x[j][3] * 0.0625f);
+                    qf[j][nt][2] = pack2<false>(x[j][4], x[j][5]);
+                    qf[j][nt][3] = pack2<false>(x[j][6] * 0.0625f, x[j][7] * 0.0625f);
                 }
-                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-                if (c == j) mine = sum;
+                split2<BF16>(make_float2(0.f, mine), qs[nt][0], qs[nt][1]);
+                const float fm = p.scale_log2 * exp2_int(eq);
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    qf[j][i][0] = pack2<false>(x[j][4 * i], x[j][4 * i + 1]);
-                    qf[j][i][1] = pack2<false>(x[j][4 * i + 2] * 0.0625f, x[j][4 * i + 3] * 0.0625f);
+                for (int e = 0; e < 2; ++e) {
+                    const int rw = 8 * nt + 2 * c + e;
+                    f_row[nt][e] = __shfl_sync(0xffffffffu, fm, (2 * c + e) * 4);  // a lane of row rw
+                    // Padding rows see the whole context: only rows that exist mask.
+                    lim[nt][e] = rw < p.rows ? ctx - p.lq + ((rw * p.group_inv) >> 16) : ctx - 1;
+                    r_ref[nt][e] = kNone;
                 }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) om[nt][i] = 0.f;
+#pragma unroll
+                for (int j = 0; j < kGroups; ++j)
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[j][t][nt][e] = 0.f;
             }
-            split2<BF16>(make_float2(0.f, mine), qs[0], qs[1]);
-            const float fm = p.scale_log2 * exp2_int(eq);
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int rw = 2 * c + e;
-                f_row[e] = __shfl_sync(0xffffffffu, fm, rw * 4);  // a lane of row rw
-                // Padding rows see the whole context: only rows that exist mask.
-                lim[e] = rw < rows ? ctx - p.lq + (((row_base + rw) * p.group_inv) >> 16) : ctx - 1;
-                r_ref[e] = kNone;
-            }
-            lim_min = ctx - p.lq + ((row_base * p.group_inv) >> 16);  // the smallest: the first row's
-            y_lim = kLazyMax - float(kExpMin<BF16>);
-            s_lim = 0.f;
-            om[0] = om[1] = om[2] = om[3] = 0.f;
-#pragma unroll
-            for (int j = 0; j < kGroups; ++j)
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[j][t][e] = 0.f;
+            lim_min = ctx - p.lq;  // the smallest: row 0's
+            unit = exp2_int(kExpMax);
+            reach_lim = 0.f;
         }
         bool wrote = false;
         {
@@ -549,19 +575,18 @@ __global__ void __launch_bounds__(kThreads, kCtas) paged_attention_q4_kernel(con
             // NaN), a page outside the cache was not loaded: both read as zeros.
             const int left = ctx - (tile * kTile + tok_warp);
             const int first = (flags & kNoPage) ? 0 : left;
-            if (__any_sync(0xffffffffu, left > 0 && first < C::kWarpTokens)) {
-                for (int i = lane; i < (C::kWarpTokens - first) * (kRecord / 16); i += 32) {
+            if (__any_sync(0xffffffffu, left > 0 && first < kWarpTokens)) {
+                for (int i = lane; i < (kWarpTokens - first) * (kRecord / 16); i += 32) {
                     uint8_t* at = sm.stages[stage] + (tok_warp + first) * kRecord + i * 16;
                     *reinterpret_cast<uint4*>(at) = make_uint4(0, 0, 0, 0);
                     *reinterpret_cast<uint4*>(at + kKvBytes) = make_uint4(0, 0, 0, 0);
                 }
-                // Where two warps share a slice (9 to 16 rows) each clears it for itself, with the same zeros.
                 wrote = true;
                 __syncwarp();
             }
         }
 #pragma unroll 1
-        for (int sub = 0; sub < C::kWarpTokens; sub += 32) {
+        for (int sub = 0; sub < kWarpTokens; sub += 32) {
             const int tok_base = tile * kTile + tok_warp + sub;
             if (__any_sync(0xffffffffu, tok_base >= ctx)) break;
             // Two copies of the step, so that the common one is straight code: EDGE is a step that reaches past
@@ -571,7 +596,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) paged_attention_q4_kernel(con
             uint8_t* kb = sm.stages[stage] + (tok_warp + sub) * kRecord;
             uint8_t* vb = kb + kKvBytes;
             // ---- log2 scores x: codes and minima of S^T = K Q^T ----
-            float x[2][4];  // sub-tile of 16: token g (+ 8 for e >= 2), rows 2 c, 2 c + 1
+            float x[2][NT][4];  // sub-tile of 16: token g (+ 8 for e >= 2), rows 8 nt + 2 c, 2 c + 1
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 const uint8_t* ks = kb + u * 16 * kRecord;
@@ -580,12 +605,6 @@ __global__ void __launch_bounds__(kThreads, kCtas) paged_attention_q4_kernel(con
                 ldsm_x4(kw[1][0], kw[1][1], kw[1][2], kw[1][3], smem_u32(ks) + frag_off + 8 * kRecord);
                 const uint4 pa4 = *reinterpret_cast<const uint4*>(ks + par_off);
                 const uint4 pb4 = *reinterpret_cast<const uint4*>(ks + par_off + 8 * kRecord);
-                float xm[4];
-                {
-                    uint32_t a[4];  // word c of tokens g, g + 8, g, g + 8
-                    ldsm_x4(a[0], a[1], a[2], a[3], smem_u32(ks) + word_off);
-                    mma_zero<BF16>(xm, a, qs[0], qs[1]);
-                }
                 const uint32_t pa[4] = {pa4.x, pa4.y, pa4.z, pa4.w}, pb[4] = {pb4.x, pb4.y, pb4.z, pb4.w};
 #pragma unroll
                 for (int j = 0; j < kGroups; ++j) {
@@ -593,64 +612,79 @@ __global__ void __launch_bounds__(kThreads, kCtas) paged_attention_q4_kernel(con
                     const uint32_t a0[4] = {wa & kLo, wb & kLo, wa & kHi, wb & kHi};
                     const uint32_t a1[4] = {wa8 & kLo, wb8 & kLo, wa8 & kHi, wb8 & kHi};
                     const float sa = lo_f<BF16>(pa[j]), sb = lo_f<BF16>(pb[j]);
-                    float acc[4];
-                    mma_zero<false>(acc, a0, qf[j][0][0], qf[j][0][1]);
-                    mma<false>(acc, a1, qf[j][1][0], qf[j][1][1]);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float sc = e < 2 ? sa : sb;
-                        x[u][e] = j == 0 ? sc * acc[e] : fmaf(sc, acc[e], x[u][e]);
+                    for (int nt = 0; nt < NT; ++nt) {
+                        float acc[4];
+                        mma_zero<false>(acc, a0, qf[j][nt][0], qf[j][nt][1]);
+                        mma<false>(acc, a1, qf[j][nt][2], qf[j][nt][3]);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float sc = e < 2 ? sa : sb;
+                            x[u][nt][e] = j == 0 ? sc * acc[e] : fmaf(sc, acc[e], x[u][nt][e]);
+                        }
                     }
                 }
+                uint32_t a[4];  // word c of tokens g, g + 8, g, g + 8
+                ldsm_x4(a[0], a[1], a[2], a[3], smem_u32(ks) + word_off);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[u][e] = fmaf(x[u][e], 16777216.f, xm[e]) * f_row[e & 1];
+                for (int nt = 0; nt < NT; ++nt) {
+                    float xm[4];
+                    mma_zero<BF16>(xm, a, qs[nt][0], qs[nt][1]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[u][nt][e] = fmaf(x[u][nt][e], 16777216.f, xm[e]) * f_row[nt][e & 1];
+                }
             }
             // ---- masks; references ----
             if constexpr (EDGE) {
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (tok_base + 16 * u + g + (e >> 1) * 8 > lim[e & 1]) x[u][e] = -INFINITY;
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (tok_base + 16 * u + g + (e >> 1) * 8 > lim[nt][e & 1]) x[u][nt][e] = -INFINITY;
             }
             float y_max = -INFINITY;
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
-                y_max = fmaxf(y_max, max3f(fmaxf(x[0][e], x[0][2 + e]), x[1][e], x[1][2 + e]) - r_ref[e]);
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    y_max = fmaxf(y_max, max3f(fmaxf(x[0][nt][e], x[0][nt][2 + e]), x[1][nt][e], x[1][nt][2 + e]) - r_ref[nt][e]);
             const uint4 look = *reinterpret_cast<const uint4*>(vb + look_off);  // value parameters of token `lane`
-            const float s_max = fmaxf(max3f(lo_f<BF16>(look.x), lo_f<BF16>(look.y), lo_f<BF16>(look.z)), lo_f<BF16>(look.w));
-            if (__any_sync(0xffffffffu, y_max > y_lim || s_max > s_lim)) {
-                // Rare: raise E to the value scales of this tile, the rows' maxima to its scores.
-                float sm_all = s_max;
+            const float reach = reach_of<BF16>(look);
+            if (__any_sync(0xffffffffu, y_max > kLazyMax || reach > reach_lim)) {
+                // Rare: raise E to the value parameters of this tile, the rows' maxima to its scores.
+                float top = reach;
 #pragma unroll
-                for (int sh = 1; sh <= 16; sh <<= 1) sm_all = fmaxf(sm_all, __shfl_xor_sync(0xffffffffu, sm_all, sh));
-                float raise = 0.f;
-                if (sm_all > s_lim) {
-                    const int old = int(kLazyMax - y_lim);  // E
-                    const int en = min(max((__float_as_int(sm_all) >> 23) - 127 - 2, old), kExpMax);
-                    raise = float(en - old);
-                    y_lim = kLazyMax - float(en);
-                    s_lim = en == kExpMax ? INFINITY : exp2_int(en + 7);
+                for (int sh = 1; sh <= 16; sh <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, sh));
+                float drop = 1.f;  // 2^-(rise of E)
+                if (top > reach_lim) {
+                    const int old = 127 - (__float_as_int(unit) >> 23);  // E
+                    const int en = min(max((__float_as_int(top) >> 23) - 127 - 6, old), kExpMax);
+                    drop = exp2_int(old - en);
+                    unit = exp2_int(-en);
+                    reach_lim = en == kExpMax ? INFINITY : exp2_int(en + 11);
                 }
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    float tm = max3f(fmaxf(x[0][e], x[0][2 + e]), x[1][e], x[1][2 + e]);
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int sh = 4; sh <= 16; sh <<= 1) tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, sh));
-                    const float ro = r_ref[e];
-                    const float rn = fmaxf(ro == kNone ? kNone : ro + raise, tm == -INFINITY ? kNone : tm + (kLazyMax - y_lim));
-                    const float alpha = ro == kNone ? 0.f : fast_exp2(ro - rn);
-                    r_ref[e] = rn;
-                    om[e] *= alpha;
-                    om[2 + e] *= alpha;
+                    for (int e = 0; e < 2; ++e) {
+                        float tm = max3f(fmaxf(x[0][nt][e], x[0][nt][2 + e]), x[1][nt][e], x[1][nt][2 + e]);
 #pragma unroll
-                    for (int j = 0; j < kGroups; ++j)
+                        for (int sh = 4; sh <= 16; sh <<= 1) tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, sh));
+                        const float ro = r_ref[nt][e], rn = fmaxf(ro, tm == -INFINITY ? kNone : tm);
+                        const float alpha = ro == kNone ? 0.f : fast_exp2(ro - rn), alpha_v = alpha * drop;
+                        r_ref[nt][e] = rn;
+                        om[nt][e] *= alpha_v;
+                        om[nt][2 + e] *= alpha;
 #pragma unroll
-                        for (int t = 0; t < 2; ++t) {
-                            o[j][t][e] *= alpha;
-                            o[j][t][2 + e] *= alpha;
-                        }
-                }
+                        for (int j = 0; j < kGroups; ++j)
+#pragma unroll
+                            for (int t = 0; t < 2; ++t) {
+                                o[j][t][nt][e] *= alpha_v;
+                                o[j][t][nt][2 + e] *= alpha_v;
+                            }
+                    }
             }
             if constexpr (EDGE) {
                 // A stored non-finite value (s = m = NaN) counts for the rows that see its token only: it
@@ -663,61 +697,64 @@ __global__ void __launch_bounds__(kThreads, kCtas) paged_attention_q4_kernel(con
                     for (; bad; bad &= bad - 1) {
                         const int t = tok_base + __ffs(bad) - 1;
 #pragma unroll
-                        for (int e = 0; e < 2; ++e)
-                            if (g == 2 * j + 1 && t <= lim[e]) om[e] = __int_as_float(0x7fffffff);
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e)
+                                if (g == 2 * j + 1 && t <= lim[nt][e]) om[nt][e] = __int_as_float(0x7fffffff);
                     }
                 }
             }
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 const uint8_t* vs = vb + u * 16 * kRecord;
-                float y[4];  // probabilities
+                // P in fp16, as B operands: lane (g, c) holds row g of tokens 2 c, 2 c + 1 (+ 8); for fp16
+                // models also what the rounding left.
+                uint32_t pb[NT][2], pl[NT][2];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) y[e] = fast_exp2(x[u][e] - r_ref[e & 1]);
-                // ---- sum_t p (parameter words), sum_t p ----
-                {
-                    uint32_t pt[4];  // half-word g of tokens 2 c, 2 c + 1 (+ 8); ones
-                    ldsm_x4_t(pt[0], pt[1], pt[2], pt[3], (lane & 8) ? smem_u32(sm.ones) : smem_u32(vs) + trans_off);
-                    if constexpr (EDGE) {
-                        pt[0] = finite2<BF16>(pt[0]);
-                        pt[2] = finite2<BF16>(pt[2]);
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const float2 y = make_float2(fast_exp2(x[u][nt][2 * i] - r_ref[nt][0]),
+                                                     fast_exp2(x[u][nt][2 * i + 1] - r_ref[nt][1]));
+                        if constexpr (BF16) {
+                            pb[nt][i] = transpose8(pack2<false>(y.x, y.y));
+                        } else {
+                            uint32_t hi, lo;
+                            split2<false>(y, hi, lo);
+                            pb[nt][i] = transpose8(hi);
+                            pl[nt][i] = transpose8(lo);
+                        }
                     }
-                    uint32_t hi[2], lo[2];
-                    split2<BF16>(make_float2(y[0], y[1]), hi[0], lo[0]);
-                    split2<BF16>(make_float2(y[2], y[3]), hi[1], lo[1]);
-                    mma<BF16>(om, pt, transpose8(hi[0]), transpose8(hi[1]));
-                    mma<BF16>(om, pt, transpose8(lo[0]), transpose8(lo[1]));
+                // Half-word g of the parameters of the same tokens, times 2^-E in fp16; ones.
+                uint32_t pt[4];
+                ldsm_x4_t(pt[0], pt[1], pt[2], pt[3], (lane & 8) ? smem_u32(sm.ones) : smem_u32(vs) + trans_off);
+#pragma unroll
+                for (int i = 0; i < 4; i += 2) {
+                    if constexpr (EDGE) pt[i] = finite2<BF16>(pt[i]);
+                    pt[i] = pack2<false>(lo_f<BF16>(pt[i]) * unit, hi_f<BF16>(pt[i]) * unit);
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    mma<false>(om[nt], pt, pb[nt][0], pb[nt][1]);
+                    if constexpr (!BF16) mma<false>(om[nt], pt, pl[nt][0], pl[nt][1]);
                 }
                 // ---- O^T += V^T (P s)^T ----
                 uint32_t vw[2][kGroups];  // half-word g of tokens 2 c, 2 c + 1 (+ 8)
                 ldsm_x4_t(vw[0][0], vw[0][1], vw[0][2], vw[0][3], smem_u32(vs) + frag_off);
                 ldsm_x4_t(vw[1][0], vw[1][1], vw[1][2], vw[1][3], smem_u32(vs) + frag_off + 8 * kRecord);
-                const uint4 pa4 = *reinterpret_cast<const uint4*>(vs + par_off);
-                const uint4 pb4 = *reinterpret_cast<const uint4*>(vs + par_off + 8 * kRecord);
-                uint32_t pa[4] = {pa4.x, pa4.y, pa4.z, pa4.w}, pb[4] = {pb4.x, pb4.y, pb4.z, pb4.w};
-                if constexpr (EDGE) {
-#pragma unroll
-                    for (int j = 0; j < kGroups; ++j) {
-                        pa[j] = finite2<BF16>(pa[j]);
-                        pb[j] = finite2<BF16>(pb[j]);
-                    }
-                }
 #pragma unroll
                 for (int j = 0; j < kGroups; ++j) {
-                    uint32_t b[2], bl[2];
-                    const float sa = lo_f<BF16>(pa[j]), sb = lo_f<BF16>(pb[j]);
-                    const float2 p0 = make_float2(y[0] * sa, y[1] * sa), p1 = make_float2(y[2] * sb, y[3] * sb);
-                    if constexpr (BF16) {
-                        b[0] = transpose8(pack2<false>(p0.x, p0.y));
-                        b[1] = transpose8(pack2<false>(p1.x, p1.y));
-                    } else {
-                        uint32_t hi[2], lo[2];
-                        split2<false>(p0, hi[0], lo[0]);
-                        split2<false>(p1, hi[1], lo[1]);
+                    // The scales of group j: half-word 2 j, from the lanes of row 2 j.
+                    uint32_t b[NT][2], bl[NT][2];
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            b[i] = transpose8(hi[i]);
-                            bl[i] = transpose8(lo[i]);
+                    for (int i = 0; i < 2; ++i) {
+                        const uint32_t sc = __shfl_sync(0xffffffffu, pt[2 * i], 8 * j + c);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            b[nt][i] = mul_f16x2(pb[nt][i], sc);
+                            // What rounding p s to fp16 left (the fused residual is exact).
+                            if constexpr (!BF16)
+                                bl[nt][i] = fma_f16x2(pl[nt][i], sc, fma_f16x2(pb[nt][i], sc, b[nt][i] ^ 0x80008000u));
                         }
                     }
 #pragma unroll
@@ -726,8 +763,11 @@ __global__ void __launch_bounds__(kThreads, kCtas) paged_attention_q4_kernel(con
                         const uint32_t w0 = t ? __byte_perm(vw[0][j], 0, 0x4341) : vw[0][j] & 0x00ff00ffu;
                         const uint32_t w1 = t ? __byte_perm(vw[1][j], 0, 0x4341) : vw[1][j] & 0x00ff00ffu;
                         const uint32_t a[4] = {w0 & kLo, w0, w1 & kLo, w1};
-                        mma<false>(o[j][t], a, b[0], b[1]);
-                        if constexpr (!BF16) mma<false>(o[j][t], a, bl[0], bl[1]);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            mma<false>(o[j][t][nt], a, b[nt][0], b[nt][1]);
+                            if constexpr (!BF16) mma<false>(o[j][t][nt], a, bl[nt][0], bl[nt][1]);
+                        }
                     }
                 }
             }
@@ -743,82 +783,86 @@ __global__ void __launch_bounds__(kThreads, kCtas) paged_attention_q4_kernel(con
         if (!__any_sync(0xffffffffu, flags & kLast)) continue;
 
         // ---- combine the warps' states of this item ----
-        // O = 2^24 o + sum p m; n' is a sixteenth of the byte's sum less the low nibble's.
+        // O = 2^E (2^24 o + sum p m); n' is a sixteenth of the byte's sum less the low nibble's.
+        const float back = __int_as_float(0x7f000000 - __float_as_int(unit));  // 2^E
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int j = 0; j < kGroups; ++j) {
-                const float mj = __shfl_sync(0xffffffffu, om[e], (2 * j + 1) * 4 + c);
+            for (int e = 0; e < 2; ++e)
 #pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    o[j][t][2 + e] = fmaf(o[j][t][2 + e] - o[j][t][e], 1048576.f, mj);
-                    o[j][t][e] = fmaf(o[j][t][e], 16777216.f, mj);
+                for (int j = 0; j < kGroups; ++j) {
+                    const float mj = __shfl_sync(0xffffffffu, om[nt][e], (2 * j + 1) * 4 + c);
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        o[j][t][nt][2 + e] = fmaf(o[j][t][nt][2 + e] - o[j][t][nt][e], 1048576.f, mj) * back;
+                        o[j][t][nt][e] = fmaf(o[j][t][nt][e], 16777216.f, mj) * back;
+                    }
                 }
-            }
-        // Dimension of o[j][t][e] for e < 2; e >= 2 is the next nibble, two dimensions on.
+        // Dimension of o[j][t][.][e] for e < 2; e >= 2 is the next nibble, two dimensions on.
         const int d0 = 8 * (g >> 1) + (g & 1);
         const bool single = hd.nch == 1;
         const int64_t slot = 2 * int64_t(blockIdx.x) + (int(blockIdx.x) == hd.first ? 1 : 0);
-        const int w0 = (warp / C::kSlices) * C::kSlices;  // first warp of this group of rows
         bool ok = true;
 #pragma unroll
-        for (int r0 = 0; r0 < 8; r0 += C::kPassRows) {
-            if (r0 >= p.rows || !ok) break;  // the first group's rows: the same passes for all warps
-            const int nr = min(C::kPassRows, rows - r0);
+        for (int r0 = 0; r0 < 8 * NT; r0 += C::kPassRows) {
+            if (r0 >= p.rows || !ok) break;
+            const int nr = min(C::kPassRows, p.rows - r0);
             if (reading) ok = consumer_wait(&sm.cbar, cphase, p.wait_ns);
             if (!ok) break;
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int r = 2 * c + e - r0;
-                if (r >= 0 && r < nr) {
-                    if (g == 0) {
-                        sm.cm[warp][r] = r_ref[e];
-                        sm.cl[warp][r] = om[2 + e];
-                    }
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int j = 0; j < kGroups; ++j)
-#pragma unroll
-                        for (int t = 0; t < 2; ++t) {
-                            float* cp = &sm.co[warp][r][32 * j + 4 * t + d0];
-                            cp[0] = o[j][t][e];
-                            cp[2] = o[j][t][2 + e];
+                for (int e = 0; e < 2; ++e) {
+                    const int r = 8 * nt + 2 * c + e - r0;
+                    if (r >= 0 && r < nr) {
+                        if (g == 0) {
+                            sm.cm[warp][r] = r_ref[nt][e];
+                            sm.cl[warp][r] = om[nt][2 + e];
                         }
+#pragma unroll
+                        for (int j = 0; j < kGroups; ++j)
+#pragma unroll
+                            for (int t = 0; t < 2; ++t) {
+                                float* cp = &sm.co[warp][r][32 * j + 4 * t + d0];
+                                cp[0] = o[j][t][nt][e];
+                                cp[2] = o[j][t][nt][2 + e];
+                            }
+                    }
                 }
-            }
             mbar_arrive(&sm.cbar);
             ok = consumer_wait(&sm.cbar, cphase, p.wait_ns);
             if (!ok) break;
-            // This warp's share of the pass's elements, two neighbours per lane and round.
-            const int n = nr * (kD / C::kSlices);
+            // A quarter of the pass's elements each, two neighbours per lane and round.
+            const int n = nr * (kD / kWarps);
             for (int i = 2 * lane; i < n; i += 64) {
-                const int el = (warp - w0) * n + i, r = el >> 7, d = el & (kD - 1);
-                float M = sm.cm[w0][r];
+                const int el = warp * n + i, r = el >> 7, d = el & (kD - 1);
+                float M = sm.cm[0][r];
 #pragma unroll
-                for (int w = 1; w < C::kSlices; ++w) M = fmaxf(M, sm.cm[w0 + w][r]);
+                for (int w = 1; w < kWarps; ++w) M = fmaxf(M, sm.cm[w][r]);
                 float den = 0.f, a0 = 0.f, a1 = 0.f;
 #pragma unroll
-                for (int w = 0; w < C::kSlices; ++w) {
-                    const float sc = fast_exp2(sm.cm[w0 + w][r] - M);
-                    den = fmaf(sm.cl[w0 + w][r], sc, den);
-                    a0 = fmaf(sm.co[w0 + w][r][d], sc, a0);
-                    a1 = fmaf(sm.co[w0 + w][r][d + 1], sc, a1);
+                for (int w = 0; w < kWarps; ++w) {
+                    const float sc = fast_exp2(sm.cm[w][r] - M);
+                    den = fmaf(sm.cl[w][r], sc, den);
+                    a0 = fmaf(sm.co[w][r][d], sc, a0);
+                    a1 = fmaf(sm.co[w][r][d + 1], sc, a1);
                 }
                 const float inv = den == 0.f ? 0.f : __fdividef(1.f, den);  // 0: the row sees no token of this item
-                const int row = row_base + r0 + r;
+                const int row = r0 + r;
                 if (single)
                     *reinterpret_cast<uint32_t*>(p.out + out_row(p, hd.b, hd.h, row) + d) = pack2<BF16>(a0 * inv, a1 * inv);
                 else
                     *reinterpret_cast<float2*>(p.part_o + (slot * p.rows + row) * kD + d) = make_float2(a0 * inv, a1 * inv);
             }
             if (!single && lane < nr) {
-                float M = sm.cm[w0][lane];
+                float M = sm.cm[0][lane];
 #pragma unroll
-                for (int w = 1; w < C::kSlices; ++w) M = fmaxf(M, sm.cm[w0 + w][lane]);
+                for (int w = 1; w < kWarps; ++w) M = fmaxf(M, sm.cm[w][lane]);
                 float den = 0.f;
 #pragma unroll
-                for (int w = 0; w < C::kSlices; ++w) den = fmaf(sm.cl[w0 + w][lane], fast_exp2(sm.cm[w0 + w][lane] - M), den);
+                for (int w = 0; w < kWarps; ++w) den = fmaf(sm.cl[w][lane], fast_exp2(sm.cm[w][lane] - M), den);
                 // A NaN sum is handed on as an infinite weight: the merge's maximum skips NaN.
-                p.part_lse[(slot * kWarps + warp) * p.rows + row_base + r0 + lane] =
+                p.part_lse[(slot * kWarps + warp) * p.rows + r0 + lane] =
                     den == 0.f ? -INFINITY : (den <= FLT_MAX ? M + fast_log2(den) : INFINITY);
             }
             mbar_arrive(&sm.cbar);
@@ -829,30 +873,36 @@ __global__ void __launch_bounds__(kThreads, kCtas) paged_attention_q4_kernel(con
             *reinterpret_cast<volatile int32_t*>(&sm.err) = 1;
             break;
         }
-        if (!single) {
-            // Publish this warp's share of the chunk (one release fence per warp, cumulative over the warp
-            // barrier), then count it; the last chunk's warp of this number merges the share.
-            __syncwarp();
-            int last = 0;
-            int32_t* counter = &p.counters[hd.first * kWarps + warp];
-            if (lane == 0) {
-                __threadfence();
-                last = atomicAdd(counter, 1) == hd.nch - 1;
-                if (last) __threadfence();
-            }
-            if (__shfl_sync(0xffffffffu, last, 0)) {
-                merge_share<BF16, ROWS16>(p, hd, row_base, rows, warp, lane);
-                if (lane == 0) *counter = 0;
-            }
+        if (!single && lane == 0) sm.part[warp][slot & 1] = hd;
+    }
+
+    // The run's partial items (its first and its last), after the loop so that the merge's registers are
+    // not held beside it: publish this warp's share of each (one release fence per warp, cumulative over the
+    // warp barrier), then count it; the last chunk's warp of this number merges the share.
+    __syncwarp();
+#pragma unroll 1
+    for (int i = 0; i < 2; ++i) {
+        const Header hd = sm.part[warp][i];
+        if (hd.nch == 0) continue;
+        int last = 0;
+        int32_t* counter = &p.counters[hd.first * kWarps + warp];
+        if (lane == 0) {
+            __threadfence();
+            last = atomicAdd(counter, 1) == hd.nch - 1;
+            if (last) __threadfence();
+        }
+        if (__shfl_sync(0xffffffffu, last, 0)) {
+            merge_share<BF16, NT>(p, hd, warp, lane);
+            if (lane == 0) *counter = 0;
         }
     }
 }
 
-template <bool BF16, bool ROWS16>
+template <bool BF16, int NT>
 void launch(const Params& prm, int ctas, cudaStream_t s) {
-    const void* fn = (const void*)paged_attention_q4_kernel<BF16, ROWS16>;
-    ensure_smem_attr(fn, int(sizeof(Smem<ROWS16>)));
-    paged_attention_q4_kernel<BF16, ROWS16><<<ctas, kThreads, sizeof(Smem<ROWS16>), s>>>(prm);
+    const void* fn = (const void*)paged_attention_q4_kernel<BF16, NT>;
+    ensure_smem_attr(fn, int(sizeof(Smem<NT>)));
+    paged_attention_q4_kernel<BF16, NT><<<ctas, kThreads, sizeof(Smem<NT>), s>>>(prm);
 }
 
 }  // namespace
@@ -863,7 +913,7 @@ extern "C" size_t b200_paged_attention_q4_workspace_size(int32_t query_len, int3
     using namespace b200::pq4;
     if (query_len < 1 || group_size < 1) return 0;
     const int64_t rows = int64_t(query_len) * group_size;
-    return rows > 16 ? 0 : workspace_bytes(int(rows), grid_ctas());
+    return rows > 16 ? 0 : workspace_bytes(int(rows));
 }
 
 extern "C" int32_t b200_paged_attention_q4(void* out, const void* q, int64_t q_stride_token, const void* k_cache,
@@ -910,11 +960,11 @@ extern "C" int32_t b200_paged_attention_q4(void* out, const void* q, int64_t q_s
                  "and at least Hq*D",
                  (long long)q_stride_token);
     if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) ||
-        workspace_size < workspace_bytes(int(rows), grid_ctas()))
+        workspace_size < workspace_bytes(int(rows)))
         return fail(B200_ERR_WORKSPACE, "paged_attention_q4: workspace missing, unaligned or smaller than %zu bytes",
-                    workspace_bytes(int(rows), grid_ctas()));
+                    workspace_bytes(int(rows)));
 
-    const int ctas = grid_ctas();
+    const int ctas = grid_ctas(int(rows));
     Params prm;
     prm.q = static_cast<const uint16_t*>(q);
     prm.q_stride = q_stride_token;
@@ -944,11 +994,11 @@ extern "C" int32_t b200_paged_attention_q4(void* out, const void* q, int64_t q_s
 
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (dtype == B200_BF16) {
-        if (rows > 8) launch<true, true>(prm, ctas, s);
-        else launch<true, false>(prm, ctas, s);
+        if (rows > 8) launch<true, 2>(prm, ctas, s);
+        else launch<true, 1>(prm, ctas, s);
     } else {
-        if (rows > 8) launch<false, true>(prm, ctas, s);
-        else launch<false, false>(prm, ctas, s);
+        if (rows > 8) launch<false, 2>(prm, ctas, s);
+        else launch<false, 1>(prm, ctas, s);
     }
     B200_CUDA_TRY(cudaGetLastError());
     return B200_OK;

@@ -88,8 +88,8 @@ def values(rec, bf16):
 def attention(q, k_rec, v_rec, block_tables, context_lens, scale, bf16):
     """q float64 [B, Lq, Hq, 128]; caches uint8 [NB, Hkv, bs, 80]; float64 [B, Lq, Hq, 128].
 
-    Also returns a bound on the error a kernel with fp32 scores and fp16 (p * s) may make before
-    it rounds its output, per element (see tolerance())."""
+    Also returns a bound on the error a kernel with fp32 scores and fp16 probabilities may make
+    before it rounds its output, per element (see tolerance())."""
     B, lq, hq, d = q.shape
     nb, hkv, bs, _ = k_rec.shape
     g = hq // hkv
@@ -120,9 +120,11 @@ def attention(q, k_rec, v_rec, block_tables, context_lens, scale, bf16):
             mag = np.einsum("hgjd,hnj->hgn", np.abs(qi).reshape(hkv, g, 4, 32),
                             15 * np.abs(sk[:, :m]) + np.abs(mk[:, :m])) * scale
             delta = mag.max(-1) * 2.0 ** -20                                          # [hkv, g]
-            reach = (15 * np.abs(sv[:, :m]) + np.abs(mv[:, :m])).max((1, 2))          # [hkv]
-            span = (15 * np.abs(sv[:, :m])).max((1, 2))
-            e = 2 * delta * reach[:, None] + (span * (2.0 ** -12 + m * 2.0 ** -27) + reach * 2.0 ** -20)[:, None]
+            reach = np.maximum((15 * np.abs(sv[:, :m]) + np.abs(mv[:, :m])).max((1, 2)),
+                               np.maximum(16 * np.abs(sv[:, :m]), np.abs(mv[:, :m])).max((1, 2)))  # [hkv]
+            span = (15 * np.abs(sv[:, :m])).max((1, 2)) if bf16 else np.zeros(hkv)
+            e = (2 * delta * reach[:, None]
+                 + (reach * (2.0 ** -11 + m * 2.0 ** -24 + m * 2.0 ** -27 + 2.0 ** -20) + span * 2.0 ** -11)[:, None])
             bound[b, i] = np.repeat(e.reshape(hq, 1), d, 1)
     return out, bound
 
@@ -130,8 +132,15 @@ def attention(q, k_rec, v_rec, block_tables, context_lens, scale, bf16):
 def tolerance(want, bound, bf16):
     """Largest error of an output: half a step of its 16-bit type, and the kernel's own bound.
 
-    The bound's terms: a relative error of 2^-20 of the scores' magnitude changes a weighted mean
-    of values by at most twice that times the largest value; p * s rounded to fp16 (2^-12 of at most 15 s;
-    2^-25 absolute below 2^-14, in units of at least a quarter of the largest scale, over m tokens);
-    2^-20 for the fp32 sums and exponentials."""
+    The bound's terms, with R the largest |value| a row may meet:
+      * a relative error of 2^-20 of the scores' magnitude changes a weighted mean of values by at
+        most twice that times R;
+      * probabilities rounded to fp16, in the numerator and the sum alike: a mean over changed
+        weights moves by at most sum |change| |v - mean| / sum p.  Half a step of fp16 is 2^-11
+        of p, and the mean absolute deviation of values in [-R, R] is at most R: 2^-11 R.  Below
+        2^-14 the step is absolute, half of it 2^-25, each of m tokens off the mean by at most
+        2 R, the sum at least 1 (the running maximum's own p): m 2^-24 R;
+      * p s rounded to fp16 before it meets codes up to 15 (bf16 models; fp16 ones keep the rest):
+        2^-11 of at most 15 s, and below 2^-14 half of 2^-24 in units of at most R / 64: m 2^-27 R;
+      * 2^-20 R for the fp32 sums and exponentials."""
     return np.abs(want) * (2.0 ** -8 if bf16 else 2.0 ** -11) + bound + (2.0 ** -130 if bf16 else 2.0 ** -25)
