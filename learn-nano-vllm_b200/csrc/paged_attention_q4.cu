@@ -91,10 +91,13 @@ struct Params {
     float* part_lse;  // [2 * CTAs][kWarps][rows]
 };
 
-// What a tile's warps need, and what is only needed at the end of an item.
-struct Header {
-    int32_t tile, flags, ctx, b;
-    int32_t h, first, nch, pad;  // CTA of the pair's first chunk, number of chunks
+// What a tile's warps need.
+struct alignas(16) TileHeader {
+    int32_t tile, flags, ctx, pad;
+};
+// What is needed at the end of an item: its pair, the CTA of the pair's first chunk, the number of chunks.
+struct alignas(16) Header {
+    int32_t b, h, first, nch;
 };
 enum : int32_t { kFirst = 1, kLast = 2, kNoPage = 4, kQBuf = 8 };
 
@@ -128,7 +131,8 @@ struct Smem {
     float cm[kWarps][Cfg<NT>::kPassRows];
     float cl[kWarps][Cfg<NT>::kPassRows];
     alignas(16) uint32_t ones[4];  // a row of fp16 ones
-    Header hdr[kStages];
+    TileHeader tile[kStages];
+    Header item[kStages];          // with an item's last tile
     Header part[kWarps][2];        // the run's partial items, as each warp left them
     uint64_t full[kStages];
     uint64_t empty[kStages];
@@ -375,22 +379,37 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
             int t = begin - at;
             // The next sequence's length and the next tile's page are loaded one step ahead.
             int ctx_next = p.context_lens[min(b + 1, p.batch - 1)];
-            auto page_of = [&](int seq, int tile) { return p.block_tables[seq * p.bt_stride + (tile * kTile) / p.block_size]; };
+            const int64_t head_bytes = int64_t(p.block_size) * kRecord, page_bytes = p.hkv * head_bytes;
+            const int32_t* table = p.block_tables + b * p.bt_stride;
+            int page = 0, off = 0;  // of tile t
+            Header item{b, h, 0, 0};
             // The first tile of the next pair that has one, if it lies in this run.
-            auto next_pair = [&](int& b, int& h, int& t, int& nt, int& ctx, int& at) {
-                t = 0;
+            auto next_pair = [&] {
+                t = page = off = 0;
                 at += span_of(nt);
-                if (at >= end || ++h < p.hkv) return;
-                h = 0;
-                do {
-                    ++b;
-                    ctx = min(ctx_next, cap);
-                    nt = tiles_of(ctx, cap);
-                    ctx_next = p.context_lens[min(b + 1, p.batch - 1)];
-                } while (nt == 0);
+                if (at >= end) return;
+                if (++item.h == p.hkv) {
+                    item.h = 0;
+                    do {
+                        ++item.b;
+                        ctx = min(ctx_next, cap);
+                        nt = tiles_of(ctx, cap);
+                        ctx_next = p.context_lens[min(item.b + 1, p.batch - 1)];
+                    } while (nt == 0);
+                    table = p.block_tables + item.b * p.bt_stride;
+                }
+                item.first = at / quota;
+                item.nch = (at + nt - 1) / quota - item.first + 1;
             };
-            if (t >= nt) next_pair(b, h, t, nt, ctx, at);
-            int blk = at + t < end ? page_of(b, t) : 0;
+            if (t < nt) {
+                page = t * kTile / p.block_size;
+                off = t * kTile - page * p.block_size;
+                item.first = at / quota;
+                item.nch = (at + nt - 1) / quota - item.first + 1;
+            } else {
+                next_pair();
+            }
+            int blk = at + t < end ? table[page] : 0;
 
             int stage = 0, qb = 0;
             uint32_t phase = 0;
@@ -399,11 +418,15 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
             bool ok = true;
             int first_flag = kFirst;
             while (at + t < end) {
+                const Header cur = item;
+                const int tile = t, tile_ctx = ctx, tile_off = off, tile_blk = blk;
                 // Where the walk goes next.
-                int b2 = b, h2 = h, t2 = t + 1, nt2 = nt, ctx2 = ctx, at2 = at;
-                if (t2 == nt) next_pair(b2, h2, t2, nt2, ctx2, at2);
-                const bool more = at2 + t2 < end, last = at2 != at || !more;
-                const int blk2 = more ? page_of(b2, t2) : 0;
+                off += kTile;
+                if (off == p.block_size) off = 0, ++page;
+                const bool pair_end = ++t == nt;
+                if (pair_end) next_pair();
+                const bool more = at + t < end, last = pair_end || !more;
+                if (more) blk = table[page];
                 if (!mbar_wait(&sm.empty[stage], phase ^ 1, p.wait_ns)) {
                     ok = false;
                     break;
@@ -417,25 +440,20 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
                     }
                     q_fill[qb] = fills;
                 }
-                const bool page = blk >= 0 && blk < p.num_blocks;
-                Header& hd = sm.hdr[stage];
-                hd.tile = t;
-                hd.flags = first_flag | (last ? kLast : 0) | (page ? 0 : kNoPage) | (qb ? kQBuf : 0);
-                hd.ctx = ctx;
-                hd.b = b;
-                hd.h = h;
-                hd.first = at / quota;
-                hd.nch = (at + nt - 1) / quota - hd.first + 1;
+                const bool in_cache = tile_blk >= 0 && tile_blk < p.num_blocks;
+                *reinterpret_cast<int4*>(&sm.tile[stage]) = make_int4(
+                    tile, first_flag | (last ? kLast : 0) | (in_cache ? 0 : kNoPage) | (qb ? kQBuf : 0), tile_ctx, 0);
+                if (last) *reinterpret_cast<int4*>(&sm.item[stage]) = make_int4(cur.b, cur.h, cur.first, cur.nch);
                 mbar_arrive_expect_tx(&sm.full[stage],
-                                      (page ? uint32_t(kStageBytes) : 0u) + (first_flag ? q_bytes * p.lq : 0u));
-                uint8_t* st = sm.stages[stage];
-                if (page) {
-                    const int64_t o = ((int64_t(blk) * p.hkv + h) * p.block_size + (t * kTile) % p.block_size) * kRecord;
+                                      (in_cache ? uint32_t(kStageBytes) : 0u) + (first_flag ? q_bytes * p.lq : 0u));
+                if (in_cache) {
+                    uint8_t* st = sm.stages[stage];
+                    const int64_t o = tile_blk * page_bytes + cur.h * head_bytes + tile_off * kRecord;
                     bulk_load_hint(st, p.k + o, kKvBytes, &sm.full[stage], pol);
                     bulk_load_hint(st + kKvBytes, p.v + o, kKvBytes, &sm.full[stage], pol);
                 }
                 if (first_flag) {
-                    const uint16_t* qsrc = p.q + int64_t(b) * p.lq * p.q_stride + int64_t(h) * p.group * kD;
+                    const uint16_t* qsrc = p.q + int64_t(cur.b) * p.lq * p.q_stride + int64_t(cur.h) * p.group * kD;
                     for (int j = 0; j < p.lq; ++j)
                         bulk_load(sm.qbuf[qb] + j * q_bytes, qsrc + int64_t(j) * p.q_stride, q_bytes, &sm.full[stage]);
                 }
@@ -443,11 +461,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
                 if (++stage == kStages) { stage = 0; phase ^= 1; }
                 first_flag = last ? kFirst : 0;
                 if (last) qb ^= 1;
-                b = b2, h = h2, t = t2, nt = nt2, ctx = ctx2, at = at2, blk = blk2;
             }
             if (ok) {
                 if (mbar_wait(&sm.empty[stage], phase ^ 1, p.wait_ns)) {
-                    sm.hdr[stage].tile = -1;  // sentinel: no more tiles
+                    sm.tile[stage].tile = -1;  // sentinel: no more tiles
                     mbar_arrive(&sm.full[stage]);
                 } else {
                     ok = false;
@@ -501,7 +518,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
             *reinterpret_cast<volatile int32_t*>(&sm.err) = 1;
             break;
         }
-        const int tile = sm.hdr[stage].tile, flags = sm.hdr[stage].flags, ctx = sm.hdr[stage].ctx;
+        const int4 head = *reinterpret_cast<const int4*>(&sm.tile[stage]);
+        const int tile = head.x, flags = head.y, ctx = head.z;
         // Votes tell the compiler that these branches are uniform.
         if (__any_sync(0xffffffffu, tile < 0)) break;
         if (__any_sync(0xffffffffu, flags & kFirst)) {
@@ -776,11 +794,13 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
             else step(std::false_type{});
         }
         if (wrote) fence_proxy_async_smem();
-        const Header hd = sm.hdr[stage];
+        const bool item_end = __any_sync(0xffffffffu, flags & kLast);
+        Header hd{0, 0, 0, 0};
+        if (item_end) hd = sm.item[stage];
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.empty[stage]);
         if (++stage == kStages) { stage = 0; phase ^= 1; }
-        if (!__any_sync(0xffffffffu, flags & kLast)) continue;
+        if (!item_end) continue;
 
         // ---- combine the warps' states of this item ----
         // O = 2^E (2^24 o + sum p m); n' is a sixteenth of the byte's sum less the low nibble's.
