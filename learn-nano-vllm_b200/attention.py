@@ -9,12 +9,17 @@ bound, then runs causal varlen prefill (over the cache when the context
 carries block tables, i.e. a prefix-cache hit or a chunked-prefill
 continuation) or paged decode.  Output shapes match the reference:
 [T, Hq, D] for prefill, [B, 1, Hq, D] for decode.
+
+Caches of dtype uint8 are 4-bit caches (quant_cache.py; install(kv_cache_bits=4) binds
+them): keys and values are quantised as they are stored, decode attends to the records,
+and a prefill that continues a cached prefix reads its sequences back first.
 """
 import torch
 from torch import nn
 
 from . import context as _ctx
 from .ops import flash_attn_varlen_func, flash_attn_with_kvcache, qk_norm_rope_store, store_kvcache
+from .quant_cache import flash_attn_with_kvcache_q4, gather_kvcache_q4, store_kvcache_q4
 
 # Where forward() reads the metadata from; integrate.install() rebinds it to
 # the reference's nanovllm.utils.context.get_context.
@@ -24,6 +29,16 @@ _get_context = _ctx.get_context
 def set_context_source(fn):
     global _get_context
     _get_context = fn
+
+
+# Rows of packed keys and values (8 heads: 512 bytes each) that a bound on their number may waste.
+_MAX_BOUND = 1 << 16
+
+
+def _total_bound(ctx):
+    """A host-side bound on cu_seqlens_k[-1], or None (one synchronising read) where it would be a large one."""
+    bound = (ctx.cu_seqlens_k.numel() - 1) * int(ctx.max_seqlen_k)
+    return bound if bound <= _MAX_BOUND else None
 
 
 class Attention(nn.Module):
@@ -40,8 +55,12 @@ class Attention(nn.Module):
         ctx = _get_context()
         cache_bound = self.k_cache.numel() > 0 and self.v_cache.numel() > 0
         if cache_bound:
-            store_kvcache(k, v, self.k_cache, self.v_cache, ctx.slot_mapping)
+            store = store_kvcache_q4 if self._quantised() else store_kvcache
+            store(k, v, self.k_cache, self.v_cache, ctx.slot_mapping)
         return self._attend(ctx, q, k, v)
+
+    def _quantised(self) -> bool:
+        return self.k_cache.dtype == torch.uint8
 
     def forward_fused(self, qkv: torch.Tensor, positions: torch.Tensor, q_norm, k_norm,
                       rotary_emb) -> torch.Tensor:
@@ -53,6 +72,11 @@ class Attention(nn.Module):
         """
         ctx = _get_context()
         cache_bound = self.k_cache.numel() > 0 and self.v_cache.numel() > 0
+        if cache_bound and self._quantised():  # the store quantises rows of the norm and the rotation
+            q, k, v = qk_norm_rope_store(qkv, positions, self.num_heads, self.num_kv_heads, q_norm.weight,
+                                         k_norm.weight, q_norm.eps, rotary_emb.cos_sin_cache)
+            store_kvcache_q4(k, v, self.k_cache, self.v_cache, ctx.slot_mapping)
+            return self._attend(ctx, q, k, v)
         need_k = ctx.is_prefill and (ctx.block_tables is None or not cache_bound)
         q, k, v = qk_norm_rope_store(qkv, positions, self.num_heads, self.num_kv_heads, q_norm.weight,
                                      k_norm.weight, q_norm.eps, rotary_emb.cos_sin_cache,
@@ -61,6 +85,17 @@ class Attention(nn.Module):
         return self._attend(ctx, q, k, v)
 
     def _attend(self, ctx, q, k, v):
+        if self._quantised():
+            if not ctx.is_prefill:
+                return flash_attn_with_kvcache_q4(q.unsqueeze(1), self.k_cache, self.v_cache,
+                                                  cache_seqlens=ctx.context_lens, block_table=ctx.block_tables,
+                                                  softmax_scale=self.scale, causal=True)
+            if ctx.block_tables is not None:
+                k, v = gather_kvcache_q4(self.k_cache, self.v_cache, ctx.cu_seqlens_k, ctx.block_tables,
+                                         _total_bound(ctx), q.dtype)
+            return flash_attn_varlen_func(q, k, v, cu_seqlens_q=ctx.cu_seqlens_q, cu_seqlens_k=ctx.cu_seqlens_k,
+                                          max_seqlen_q=ctx.max_seqlen_q, max_seqlen_k=ctx.max_seqlen_k,
+                                          softmax_scale=self.scale, causal=True)
         if not ctx.is_prefill:
             return flash_attn_with_kvcache(q.unsqueeze(1), self.k_cache, self.v_cache,
                                            cache_seqlens=ctx.context_lens, block_table=ctx.block_tables,

@@ -131,6 +131,35 @@ def _allreduce_row_parallel_forward(self, x):
     return y
 
 
+_ORIGINAL_ALLOCATE = []
+
+
+def _q4_allocate_kv_cache(self):
+    """ModelRunner.allocate_kv_cache (nanovllm/engine/model_runner.py:103-121) for 4-bit caches: the same
+    share of the device memory, in blocks of 80 instead of 256 bytes per (token, kv head) and cache."""
+    from .quant_cache import q4_cache_shape
+    cfg, hf = self.config, self.config.hf_config
+    heads = hf.num_key_value_heads // self.world_size
+    head_dim = getattr(hf, "head_dim", None) or hf.hidden_size // hf.num_attention_heads
+    if self.block_size % 128 or hf.num_attention_heads // hf.num_key_value_heads > 16:
+        raise NotImplementedError(f"4-bit KV cache: block_size {self.block_size} (a multiple of 128), "
+                                  f"{hf.num_attention_heads} heads over {hf.num_key_value_heads} (at most 16 per kv head)")
+    block = torch.Size(q4_cache_shape(1, self.block_size, heads, head_dim)).numel()
+    layers = [m for m in self.model.modules() if hasattr(m, "k_cache") and hasattr(m, "v_cache")]
+    free, total = torch.cuda.mem_get_info()
+    stats = torch.cuda.memory_stats()
+    # what stays in use, and what the largest forward needed beyond it
+    reserve = total - free + stats["allocated_bytes.all.peak"] - stats["allocated_bytes.all.current"]
+    blocks = (int(total * cfg.gpu_memory_utilization) - reserve) // (2 * len(layers) * block)
+    cfg.num_kvcache_blocks = min(blocks, (2 ** 31 - 1) // self.block_size)  # slots are int32
+    assert cfg.num_kvcache_blocks > 0, "no memory left for the KV cache"
+    # zeros: records that no token was written to are finite
+    self.kv_cache = torch.zeros(2, len(layers), *q4_cache_shape(cfg.num_kvcache_blocks, self.block_size, heads, head_dim),
+                                dtype=torch.uint8, device=torch.device("cuda", torch.cuda.current_device()))
+    for i, layer in enumerate(layers):
+        layer.k_cache, layer.v_cache = self.kv_cache[0, i], self.kv_cache[1, i]
+
+
 class _FusedSamplerState:
     """Seed and per-call offset of the fused sampler's counter-based noise."""
     seed = 0
@@ -147,7 +176,7 @@ def _fused_sampler_forward(self, logits, temperatures):
 
 def install(fuse_qk_epilogue: bool = False, fuse_sampler: bool = False, workers: bool = False,
             worker_setup: tuple = (), device_metadata: bool = False, fuse_row_parallel: bool = False,
-            row_parallel_allreduce: bool = False):
+            row_parallel_allreduce: bool = False, kv_cache_bits: int = 16):
     """Patch the importable `nanovllm` package; returns the patched modules.
 
     With fuse_qk_epilogue, Qwen3Attention.forward also runs q/k RMSNorm, RoPE and
@@ -162,11 +191,16 @@ def install(fuse_qk_epilogue: bool = False, fuse_sampler: bool = False, workers:
     it, so it implies workers.  With row_parallel_allreduce (and not fuse_row_parallel),
     RowParallelLinear.forward keeps F.linear and replaces its NCCL all-reduce with this
     package's two-shot all-reduce (allreduce.AllReduce) for decode-sized outputs; it too implies
-    workers.  With workers, the
+    workers.  With kv_cache_bits=4, ModelRunner.allocate_kv_cache binds 4-bit caches (quant_cache),
+    3.2 times the tokens in the same memory; keys and values are quantised as they are stored.  Every
+    tensor-parallel rank must allocate the same blocks, so with several ranks it needs workers.
+    With workers, the
     engine's tensor-parallel ranks (spawned processes, nanovllm/engine/llm_engine.py:24-30)
     run install() with the same options before building their ModelRunner;
     worker_setup lists "module:function" hooks they run first.
     """
+    if kv_cache_bits not in (16, 4):
+        raise NotImplementedError(f"kv_cache_bits {kv_cache_bits} (16 or 4)")
     ctx_mod = importlib.import_module("nanovllm.utils.context")
     attn_mod = importlib.import_module("nanovllm.layers.attention")
     qwen3 = importlib.import_module("nanovllm.models.qwen3")
@@ -189,6 +223,9 @@ def install(fuse_qk_epilogue: bool = False, fuse_sampler: bool = False, workers:
         _ORIGINAL_PREPARE.extend([runner_mod.ModelRunner.prepare_decode, runner_mod.ModelRunner.prepare_sample])
     runner_mod.ModelRunner.prepare_decode = _device_prepare_decode if device_metadata else _ORIGINAL_PREPARE[0]
     runner_mod.ModelRunner.prepare_sample = _device_prepare_sample if device_metadata else _ORIGINAL_PREPARE[1]
+    if not _ORIGINAL_ALLOCATE:
+        _ORIGINAL_ALLOCATE.append(runner_mod.ModelRunner.allocate_kv_cache)
+    runner_mod.ModelRunner.allocate_kv_cache = _q4_allocate_kv_cache if kv_cache_bits == 4 else _ORIGINAL_ALLOCATE[0]
     linear_mod = importlib.import_module("nanovllm.layers.linear")
     if not _ORIGINAL_ROW:
         _ORIGINAL_ROW.append(linear_mod.RowParallelLinear.forward)
@@ -201,7 +238,7 @@ def install(fuse_qk_epilogue: bool = False, fuse_sampler: bool = False, workers:
         opts = {"setup": list(worker_setup),
                 "install": {"fuse_qk_epilogue": fuse_qk_epilogue, "fuse_sampler": fuse_sampler,
                             "device_metadata": device_metadata, "fuse_row_parallel": fuse_row_parallel,
-                            "row_parallel_allreduce": row_parallel_allreduce}}
+                            "row_parallel_allreduce": row_parallel_allreduce, "kv_cache_bits": kv_cache_bits}}
         engine_mod.ModelRunner = functools.partial(entry.nanovllm_worker, options=opts)
     else:
         engine_mod.ModelRunner = runner_mod.ModelRunner
