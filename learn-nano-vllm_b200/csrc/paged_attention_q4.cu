@@ -14,31 +14,41 @@
 //     register both times.  For the values the second operand row is the byte n + 16 n' as it is:
 //     n' comes out by subtraction at the end, which saves a mask.  P^T turns into a B operand by
 //     movmatrix.
-//   * The words (s, m) of a token are an operand as they are: against the rows (0, sum(q_g)) they
-//     give the minima's part of the score; against P^T, transposed, sum_t p m, and a row of ones
-//     beside them the softmax sum.  sum(q_g) and p enter as two 16-bit parts (hi + lo).
-//   * The scales are applied in fp32, to the products with the key codes and to the probabilities;
-//     p s is rounded to fp16 for the product with the value codes (2^-12; two parts for fp16
-//     models, whose outputs would show it).
+//   * The words (s, m) of a token are operands too: against the rows (0, sum(q_g)), in two 16-bit
+//     parts, they give the minima's part of the score; taken to fp16 (times a power of two) and
+//     transposed, against P^T, sum_t p m, and with a row of ones beside them the softmax sum.
+//   * The key scales multiply the products in fp32.  The value scales multiply P^T in fp16: the
+//     lanes of row 2 g of the transposed words hold them, one shuffle hands them round.
+// Roundings: p to fp16 (2^-11), the same rounded p in the products and in the sum, so that the
+// result is a mean under weights off by as much; p s to fp16 (2^-11).  fp16 models, whose outputs
+// would show both, carry the rest of p and of p s in a second product (0.00023 from 64 bits
+// relative, 0.00034 without; the output's own rounding is 0.0002).  Sums and maxima are fp32.
 //
-// Ranges.  A row's probabilities are 2^(x - r) with r = (lazy running maximum) + E, where 2^E
-// follows the largest value scale the warp has met (raised when a scale exceeds 2^7 times it):
-// p s then stays below 2^15 and small scales do not underflow fp16.  Queries are scaled by a
-// power of two per row (largest element in [8, 16)), exactly but for elements below 2^-18 of it.
+// Ranges.  p = 2^(x - r) with r the lazily raised running maximum, so p <= 2^kLazyMax.  The value
+// parameters enter as 2^-E of themselves, where E follows the largest max(16 s, |m|) the warp has
+// met (16 s 2^-E below 2^7 when E is set, raised beyond 2^11).  Queries are scaled by a power of
+// two per row (largest element in [8, 16)), exactly but for elements below 2^-18 of it.
 //
 // Work split.  The tiles of 128 tokens of all (sequence, kv head) pairs in a row, sequence by
-// sequence, are cut into equal runs, one per CTA, all CTAs resident: no claims, no tail, a
-// sequence is split only where a run ends, and a long one over as many CTAs as its share of the
-// work.  Every CTA plans its run from context_lens (no host sync: the call can be captured).
-// A CTA leaves at most two partial results, its first and its last; the warp that finishes the
-// last chunk of a split pair (one counter per consumer warp) merges its share of the outputs.
+// sequence, are cut into equal runs (a pair counts kPairCost tiles more for its combine), one per
+// CTA, all CTAs resident: no claims, a sequence is split only where a run ends, and a long one over
+// as many CTAs as its share of the work.  Every CTA plans its run from context_lens (no host sync:
+// the call can be captured).  A CTA leaves at most two partial results, its first and its last; the
+// warp that finishes the last chunk of a split pair (one counter per consumer warp) merges its
+// share of the outputs.
 //
-// CTA.  Four consumer warps and a producer warp, three CTAs per SM (15 warps leave 128 registers
-// a thread).  A stage is 128 records of keys and 128 of values, two contiguous 10 KiB bulk copies
-// into a ring of three, guarded by full / empty mbarriers.  Up to 8 query rows each consumer warp
-// takes 32 of a tile's tokens; for 9 to 16 rows two warps take rows 0-7 and two rows 8-15, 64
-// tokens each.  The warps keep their own softmax states and combine them through shared memory at the
-// end of an item.  Every wait is bounded (kWaitLimitNs, or the test limit).
+// CTA.  Four consumer warps and a producer warp; three CTAs per SM up to 8 query rows (15 warps
+// leave 128 registers a thread), two for up to 16 (168).  A stage is 128 records of keys and 128 of
+// values, two contiguous 10 KiB bulk copies into a ring of two, guarded by full / empty mbarriers;
+// each consumer warp takes 32 of a tile's tokens, in two sub-tiles of 16.  The warps keep their own
+// softmax states and combine them through shared memory at the end of an item.  Every wait is
+// bounded (kWaitLimitNs, or the test limit).
+//
+// What bounds it (512 sequences, 1.17 M tokens, 8 kv heads of 4 rows: 1.50 GB, 228 us at the measured
+// copy rate): 280 us, 163 M warp instructions, the vector pipes; held for a second it reaches the
+// board's power cap and 320 us.  A record costs its share of 280 instructions per 16 tokens, 72 of
+// them masks.
+#include <atomic>
 #include <cfloat>
 #include <climits>
 #include <type_traits>
@@ -58,14 +68,18 @@ using q4::lo_f;
 constexpr int kTile = 128;  // tokens per stage
 constexpr int kWarps = 4;   // consumer warps
 constexpr int kWarpTokens = kTile / kWarps;
-constexpr int kQBufs = 2;   // items whose query rows fit
 constexpr int kConsumers = kWarps * 32;
 constexpr int kThreads = kConsumers + 32;
 constexpr int kStages = 2;
+// Items whose query rows fit: rows are taken with an item's first tile, so a buffer is free again when
+// the stage that is filled next is.
+constexpr int kQBufs = kStages;
 constexpr int kKvBytes = kTile * kRecord;  // keys (or values) of one stage
 constexpr int kStageBytes = 2 * kKvBytes;
 constexpr int kMaxBatch = 2048;
-constexpr int kPairCost = 2;  // what a (sequence, kv head) pair costs beside its tiles, in tiles
+// What a (sequence, kv head) pair costs beside its tiles, in tiles (decode of 512 sequences / verify of
+// 128: 280 / 134 us with 2, 281 / 142 with 1, 284 / 136 with 3, 289 / 138 with 4).
+constexpr int kPairCost = 2;
 constexpr float kLazyMax = 8.f;  // log2 headroom before a row's running maximum is raised
 constexpr float kNone = -1e30f;  // reference of a row that has met no token
 constexpr int kExpMax = 60;      // bound of |E| and of the query rows' exponents
@@ -260,7 +274,7 @@ __device__ __forceinline__ void merge_share(const Params& p, const Header& hd, i
         for (int i = 4 * lane; i < share; i += 128) {
             const int e = r0 * kD + warp * share + i, r = e >> 7, d = e & (kD - 1);
             float m = -INFINITY, den = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-                        for (int c0 = 0; c0 < hd.nch; c0 += kFlight) {
+            for (int c0 = 0; c0 < hd.nch; c0 += kFlight) {
                 float lse[kFlight];
                 float4 x[kFlight];
                 float mx = m;
@@ -414,7 +428,6 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
             int stage = 0, qb = 0;
             uint32_t phase = 0;
             int fills = 0;
-            int q_fill[2] = {-kStages, -kStages};  // fill that brought the query rows of each buffer
             bool ok = true;
             int first_flag = kFirst;
             while (at + t < end) {
@@ -430,15 +443,6 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
                 if (!mbar_wait(&sm.empty[stage], phase ^ 1, p.wait_ns)) {
                     ok = false;
                     break;
-                }
-                if (first_flag) {
-                    // The query buffer's last rows were taken with their item's first tile.
-                    const int f = q_fill[qb];
-                    if (f > fills - kStages && f >= 0 && !mbar_wait(&sm.empty[f % kStages], (f / kStages) & 1, p.wait_ns)) {
-                        ok = false;
-                        break;
-                    }
-                    q_fill[qb] = fills;
                 }
                 const bool in_cache = tile_blk >= 0 && tile_blk < p.num_blocks;
                 *reinterpret_cast<int4*>(&sm.tile[stage]) = make_int4(
@@ -921,8 +925,14 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
 
 template <bool BF16, int NT>
 void launch(const Params& prm, int ctas, cudaStream_t s) {
-    const void* fn = (const void*)paged_attention_q4_kernel<BF16, NT>;
-    ensure_smem_attr(fn, int(sizeof(Smem<NT>)));
+    // The shared-memory limit is set once per device (a call of its own costs the host as much as the
+    // argument checks); setting it twice does no harm.
+    static std::atomic<uint64_t> done{0};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64 || !(done.load(std::memory_order_relaxed) >> dev & 1)) {
+        ensure_smem_attr((const void*)paged_attention_q4_kernel<BF16, NT>, int(sizeof(Smem<NT>)));
+        if (dev < 64) done.fetch_or(uint64_t(1) << dev, std::memory_order_relaxed);
+    }
     paged_attention_q4_kernel<BF16, NT><<<ctas, kThreads, sizeof(Smem<NT>), s>>>(prm);
 }
 

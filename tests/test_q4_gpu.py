@@ -261,6 +261,34 @@ def test_several_queries(pkg, dtype, lq, hq, hkv):
     check(pkg, *make([512, 2100, 7, 1300, 2, 1, 128], hq, hkv, lq=lq, dtype=dtype, seed=lq * 10 + hkv), what=f"lq={lq} {hq}/{hkv}")
 
 
+@pytest.mark.parametrize("lq,hq,hkv", [(1, 12, 4), (3, 12, 4), (5, 12, 4), (3, 5, 1), (1, 7, 1), (2, 14, 2), (1, 13, 1), (1, 11, 1)])
+def test_odd_groups(pkg, lq, hq, hkv):
+    """Groups that are no power of two, up to 15 rows of a kv head."""
+    check(pkg, *make([260, 5, 1111], hq, hkv, lq=lq, seed=hq), what=f"{lq} {hq}/{hkv}")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_offsets_beyond_the_spread(pkg, dtype):
+    """Groups whose minimum is far larger than their range, and groups that are constant (scale 0)."""
+    q, kc, vc, cl, bt = make([700, 19], 16, 8, dtype=dtype, seed=40)
+    nb = kc.shape[0]
+    g = torch.Generator(device="cuda").manual_seed(41)
+
+    def cache(base, spread):
+        x = torch.randn(nb, 8 * 256, 128, generator=g, device="cuda") * spread
+        x[..., 32:64] = 0                                                 # a constant group
+        x[..., 64:96] += base * torch.randn(1, 1, 32, generator=g, device="cuda")
+        return torch.from_numpy(oracle_records(x.to(dtype)).reshape(nb, 8, 256, 80)).cuda()
+    check(pkg, q, cache(20.0, 0.2), cache(300.0, 0.5), cl, bt, what="offsets")
+    check(pkg, q, cache(0.0, 0.0), cache(0.0, 0.0), cl, bt, what="zeros")
+
+
+def test_many_one_tile_sequences(pkg):
+    """Hundreds of short sequences (one to 130 tokens), most items one tile, some batch rows empty."""
+    n = np.random.default_rng(0).integers(0, 131, 700)
+    check(pkg, *make(n, 4, 2, bs=128, seed=42), what="700 short")
+
+
 @pytest.mark.parametrize("bs", [128, 256, 384, 512])
 def test_block_sizes(pkg, bs):
     check(pkg, *make([1000, 385, 128, 513], 16, 8, bs=bs, seed=bs), what=f"block {bs}")
