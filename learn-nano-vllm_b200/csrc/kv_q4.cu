@@ -36,20 +36,21 @@ struct Cache {
     int64_t num_slots;
 };
 
-// Byte offset of head 0's record of a slot (heads are block_size records apart).
-__device__ __forceinline__ int64_t record_of(const Cache& c, int32_t slot) {
+// Index of head 0's record of a slot (heads are block_size records apart).  All records of a cache
+// have 32-bit indices, which leaves one multiply-add per address.
+__device__ __forceinline__ uint32_t record_of(const Cache& c, int32_t slot) {
     const uint32_t blk = uint32_t(slot) / uint32_t(c.block_size);
-    return (int64_t(blk) * c.hkv * c.block_size + (uint32_t(slot) - blk * c.block_size)) * kRecord;
+    return blk * uint32_t(c.hkv) * uint32_t(c.block_size) + (uint32_t(slot) - blk * c.block_size);
 }
 
-// Offsets of a block's tokens that have no record: rows that read as zeros, rows that are left alone.
-constexpr int64_t kZero = -1, kSkip = -2;
+// Tokens without a record: rows that read as zeros, rows that are left alone.
+constexpr uint32_t kZero = 0xffffffffu, kSkip = 0xfffffffeu;
 
 // Deals the rows of `count` tokens to the block's warps and calls, kFlight pairs at a time, LOAD and then
-// USE for each: (u, offset of the token's record, the head's records, the lane's 16 bytes of the row).
-// Both halves of a warp run together; past the last pair the offset is kSkip.
+// USE for each: (u, index of the token's record, the head's records, the lane's 16 bytes of the row).
+// Both halves of a warp run together; past the last pair the index is kSkip.
 template <int kFlight, typename LOAD, typename USE>
-__device__ __forceinline__ void for_rows(const Rows& rows, const Cache& cache, const int64_t* s_rec, int64_t t0, int count,
+__device__ __forceinline__ void for_rows(const Rows& rows, const Cache& cache, const uint32_t* s_rec, int64_t t0, int count,
                                          LOAD load, USE use) {
     const int half = (threadIdx.x >> 4) & 1, l = threadIdx.x & 15, pairs = (count + 1) >> 1;
     for (int r = blockIdx.y * kWarps + (threadIdx.x >> 5); r < 2 * cache.hkv; r += gridDim.y * kWarps) {
@@ -59,7 +60,7 @@ __device__ __forceinline__ void for_rows(const Rows& rows, const Cache& cache, c
         char* row = (v ? rows.v : rows.k) + (t0 + half) * stride + h * (kD * 2) + 16 * l;
         char* records = (v ? cache.v : cache.k) + int64_t(h) * cache.block_size * kRecord;
         for (int p0 = 0; p0 < pairs; p0 += kFlight) {
-            int64_t rec[kFlight];
+            uint32_t rec[kFlight];
 #pragma unroll
             for (int u = 0; u < kFlight; ++u) {
                 rec[u] = p0 + u < pairs ? s_rec[2 * (p0 + u) + half] : kSkip;
@@ -75,7 +76,7 @@ __device__ __forceinline__ void for_rows(const Rows& rows, const Cache& cache, c
 template <bool BF16, bool VEC, int kFlight>
 __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm)
     store_kernel(const Rows rows, const Cache cache, const int32_t* __restrict__ slots, int32_t n, int32_t tokens) {
-    __shared__ int64_t s_rec[kMaxTokens];
+    __shared__ uint32_t s_rec[kMaxTokens];
     const int64_t t0 = int64_t(blockIdx.x) * tokens;
     const int count = int(min(int64_t(tokens), n - t0));
     if (threadIdx.x < kMaxTokens) {
@@ -87,9 +88,9 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm)
     uint32_t x[kFlight][4];
     for_rows<kFlight>(
         rows, cache, s_rec, t0, count,
-        [&](int u, int64_t rec, char*, char* row) {
+        [&](int u, uint32_t rec, char*, char* row) {
             x[u][0] = x[u][1] = x[u][2] = x[u][3] = 0;
-            if (rec < 0) return;
+            if (rec >= kSkip) return;
             if constexpr (VEC) {
                 const uint4 w = __ldg(reinterpret_cast<const uint4*>(row));
                 x[u][0] = w.x, x[u][1] = w.y, x[u][2] = w.z, x[u][3] = w.w;
@@ -99,29 +100,29 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm)
                 for (int i = 0; i < 4; ++i) x[u][i] = uint32_t(e[2 * i]) | (uint32_t(e[2 * i + 1]) << 16);
             }
         },
-        [&](int u, int64_t rec, char* records, char*) {
+        [&](int u, uint32_t rec, char* records, char*) {
             uint32_t params;
             const uint32_t word = quantise8<BF16>(x[u], params);
-            if (rec < 0) return;
-            *reinterpret_cast<uint32_t*>(records + rec + 4 * l) = word;
-            if ((l & 3) == 0) *reinterpret_cast<uint32_t*>(records + rec + kParams + l) = params;
+            if (rec >= kSkip) return;
+            *reinterpret_cast<uint32_t*>(records + int64_t(rec) * kRecord + 4 * l) = word;
+            if ((l & 3) == 0) *reinterpret_cast<uint32_t*>(records + int64_t(rec) * kRecord + kParams + l) = params;
         });
 }
 
 template <bool BF16, bool VEC, int kFlight>
-__device__ __forceinline__ void read_rows(const Rows& rows, const Cache& cache, const int64_t* s_rec, int64_t t0,
+__device__ __forceinline__ void read_rows(const Rows& rows, const Cache& cache, const uint32_t* s_rec, int64_t t0,
                                           int count) {
     const int l = threadIdx.x & 15;
     uint32_t word[kFlight], params[kFlight];
     for_rows<kFlight>(
         rows, cache, s_rec, t0, count,
-        [&](int u, int64_t rec, char* records, char*) {
+        [&](int u, uint32_t rec, char* records, char*) {
             word[u] = params[u] = 0;
-            if (rec < 0) return;
-            word[u] = __ldg(reinterpret_cast<const uint32_t*>(records + rec + 4 * l));
-            params[u] = __ldg(reinterpret_cast<const uint32_t*>(records + rec + kParams + (l & ~3)));
+            if (rec >= kSkip) return;
+            word[u] = __ldg(reinterpret_cast<const uint32_t*>(records + int64_t(rec) * kRecord + 4 * l));
+            params[u] = __ldg(reinterpret_cast<const uint32_t*>(records + int64_t(rec) * kRecord + kParams + (l & ~3)));
         },
-        [&](int u, int64_t rec, char*, char* row) {
+        [&](int u, uint32_t rec, char*, char* row) {
             if (rec == kSkip) return;
             const uint4 y = dequantise8<BF16>(word[u], params[u]);  // no record: zeros
             if constexpr (VEC) {
@@ -138,11 +139,11 @@ __device__ __forceinline__ void read_rows(const Rows& rows, const Cache& cache, 
 template <bool BF16, bool VEC, int kFlight>
 __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm)
     load_kernel(const Rows rows, const Cache cache, const int32_t* __restrict__ slots, int32_t n, int32_t tokens) {
-    __shared__ int64_t s_rec[kMaxTokens];
+    __shared__ uint32_t s_rec[kMaxTokens];
     const int64_t t0 = int64_t(blockIdx.x) * tokens;
     const int count = int(min(int64_t(tokens), n - t0));
     if (threadIdx.x < kMaxTokens) {
-        int64_t rec = kSkip;
+        uint32_t rec = kSkip;
         if (threadIdx.x < count) {
             const int32_t s = slots[t0 + threadIdx.x];
             rec = s >= 0 && s < cache.num_slots ? record_of(cache, s) : kZero;
@@ -157,12 +158,12 @@ template <bool BF16, bool VEC, int kFlight>
 __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm)
     gather_kernel(const Rows rows, const Cache cache, const int32_t* __restrict__ cu, const int32_t* __restrict__ tables,
                   int64_t bt_stride, int32_t bt_width, int32_t num_seqs, int32_t n, int32_t tokens) {
-    __shared__ int64_t s_rec[kMaxTokens];
+    __shared__ uint32_t s_rec[kMaxTokens];
     const int64_t t0 = int64_t(blockIdx.x) * tokens;
     const int count = int(min(int64_t(tokens), n - t0));
     if (threadIdx.x < kMaxTokens) {
         const int32_t t = int32_t(t0) + threadIdx.x;
-        int64_t rec = kSkip;
+        uint32_t rec = kSkip;
         if (threadIdx.x < count && t >= cu[0] && t < cu[num_seqs]) {  // else: a row of no sequence
             int lo = 0, hi = num_seqs;                               // the last sequence that starts at or before t
             while (hi - lo > 1) {
@@ -217,6 +218,9 @@ int32_t check_common(const char* what, const void* k_rows, int64_t k_stride, con
         return fail(B200_ERR_UNSUPPORTED, "%s: dtype %d (bf16 or fp16 only)", what, dtype);
     B200_REQUIRE(num_blocks > 0 && block_size > 0 && int64_t(num_blocks) * block_size < (int64_t(1) << 31),
                  "%s: %d blocks of %d tokens", what, num_blocks, block_size);
+    if (int64_t(num_blocks) * block_size > int64_t(kSkip) / num_kv_heads)
+        return fail(B200_ERR_UNSUPPORTED, "%s: %d blocks of %d tokens and %d heads: more than 2^32 records", what,
+                    num_blocks, block_size, num_kv_heads);
     const int64_t row = int64_t(num_kv_heads) * kD;
     B200_REQUIRE(num_tokens <= 1 || (k_stride >= row && v_stride >= row), "%s: token stride (%lld, %lld) below Hkv*D = %lld",
                  what, (long long)k_stride, (long long)v_stride, (long long)row);
