@@ -142,11 +142,13 @@ B200_API int32_t b200_gather_kvcache_q4(void* key, int64_t key_stride,
  * masks and padding rows.  The workspace works as there
  * (b200_paged_attention_q4_workspace_size bytes for the current device,
  * 256-byte aligned, zero-filled once, whatever the batch; a call leaves its
- * counters zeroed; b200_workspace_error reads its error word).  Block tables are rows of block_table_width entries,
- * block_table_stride apart; a tile of a block id outside the cache counts as
- * tokens of zeros.  Scores, softmax statistics and sums are fp32; p * s is
- * rounded to fp16 for the product with the codes.  Queries and stored scales
- * are expected between 2^-60 and 2^60 in magnitude.
+ * counters zeroed; b200_workspace_error reads its error word).  Block tables
+ * are rows of block_table_width entries, block_table_stride apart; a tile of a
+ * block id outside the cache counts as tokens of zeros.  Scores, softmax
+ * statistics and sums are fp32; the probabilities p (and p * s, for the product
+ * with the codes) are rounded to fp16, and fp16 models add the products of what
+ * the rounding left.  Queries, stored scales and stored minima are expected
+ * between 2^-60 and 2^60 in magnitude, or zero.
  */
 B200_API size_t b200_paged_attention_q4_workspace_size(int32_t query_len, int32_t group_size);
 

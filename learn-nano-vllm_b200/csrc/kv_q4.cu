@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm)
 // More: whole waves of resident blocks, each of at most kMaxTokens tokens and four pairs per warp in
 // flight.  16,384 tokens x 8 heads, store and load: 40.0 us with whole waves of up to 24 tokens, 40.8
 // with powers of two up to 32; gather of 68.6k tokens: 55.8 against 56.9 us; 6 resident blocks of 40
-// registers lose 2 us on both and win 8 us of 114 on four sequences of 26k.
+// registers lose 2 us on both and win 8 us of 112 on four sequences of 26k.
 struct Shape {
     int tokens;
     dim3 grid;

@@ -28,6 +28,8 @@ from .ops import _DTYPES
 HEAD_DIM = 128
 RECORD_BYTES = 80
 _CONTROL_BYTES = 16384  # covers the control words and counters at the start of an attention workspace
+_U8, _I32 = torch.uint8, torch.int32
+_current_device = torch._C._cuda_getDevice
 _raw_stream = torch._C._cuda_getCurrentRawStream  # the handle that torch.cuda.current_stream wraps
 
 
@@ -40,25 +42,15 @@ def q4_cache_shape(num_blocks: int, block_size: int, num_kv_heads: int, head_dim
 
 # The checks.  A decode step makes two of these calls per layer, and for small batches the host is what
 # bounds them: each op asks once whether everything holds and only looks for the reason if it does not.
-def _cache_ok(k_cache, v_cache, num_kv_heads):
-    shape = k_cache.shape
-    return (k_cache.dtype == torch.uint8 == v_cache.dtype and len(shape) == 4 and shape[3] == RECORD_BYTES
-            and shape[1] == num_kv_heads and v_cache.shape == shape and k_cache.is_contiguous()
-            and v_cache.is_contiguous())
+def _cache_ok(k_cache, v_cache, shape):
+    return (len(shape) == 4 and shape[3] == RECORD_BYTES and k_cache.dtype is _U8 and v_cache.dtype is _U8
+            and v_cache.shape == shape and k_cache.is_contiguous() and v_cache.is_contiguous())
 
 
-def _rows_ok(key, value):
-    shape, ks, vs = key.shape, key.stride(), value.stride()
+def _rows_ok(key, value, shape, ks, vs):
     return (len(shape) == 3 and shape[2] == HEAD_DIM and value.shape == shape and key.dtype in _DTYPES
-            and value.dtype == key.dtype and ks[2] == 1 == vs[2]
-            and (shape[1] == 1 or ks[1] == HEAD_DIM == vs[1]))
-
-
-def _same_device(index, *tensors):
-    for t in tensors:
-        if t.get_device() != index:
-            return False
-    return index >= 0
+            and value.dtype is key.dtype and ks[2] == 1 and vs[2] == 1
+            and (shape[1] == 1 or (ks[1] == HEAD_DIM and vs[1] == HEAD_DIM)))
 
 
 def _refuse_type(dtype, head_dim):
@@ -93,18 +85,13 @@ def _explain_devices(*tensors):
 
 def _call(name, index, fn, *args):
     """fn(*args, stream) with device `index` current and its current stream; raises for a status."""
-    if torch._C._cuda_getDevice() == index:
+    if _current_device() == index:
         rc = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
             rc = fn(*args, _raw_stream(index))
     if rc:
         check(rc, name)
-
-
-def _token_stride(t):
-    """Token stride of [N, H, D] rows; a single row may carry any stride on its size-1 dim."""
-    return t.stride(0) if t.size(0) > 1 else t.size(1) * t.size(2)
 
 
 def store_kvcache_q4(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -114,34 +101,40 @@ def store_kvcache_q4(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tens
     Slots of -1 (padding) or outside the cache are skipped; the others must be
     unique within one call (as for `store_kvcache`).
     """
-    if not _rows_ok(key, value):
+    shape, ks, vs, cs = key.shape, key.stride(), value.stride(), k_cache.shape
+    if not _rows_ok(key, value, shape, ks, vs):
         _explain_rows(key, value)
-    N, H, _ = key.shape
-    if not _cache_ok(k_cache, v_cache, H):
+    N, H, _ = shape
+    if not (_cache_ok(k_cache, v_cache, cs) and cs[1] == H):
         _explain_cache(k_cache, v_cache, H)
-    if slot_mapping.dtype != torch.int32 or slot_mapping.numel() != N or not slot_mapping.is_contiguous():
+    if slot_mapping.dtype is not _I32 or slot_mapping.numel() != N or not slot_mapping.is_contiguous():
         _explain_ints("slot_mapping", slot_mapping)
     dev = key.get_device()
-    if not _same_device(dev, value, k_cache, v_cache, slot_mapping):
+    if not (dev >= 0 and value.get_device() == dev and k_cache.get_device() == dev and v_cache.get_device() == dev
+            and slot_mapping.get_device() == dev):
         _explain_devices(key, value, k_cache, v_cache, slot_mapping)
-    NB, _, bs, _ = k_cache.shape
-    _call("store_kvcache_q4", dev, lib().b200_store_kvcache_q4, key.data_ptr(), _token_stride(key), value.data_ptr(),
-          _token_stride(value), k_cache.data_ptr(), v_cache.data_ptr(), slot_mapping.data_ptr(), N, H, HEAD_DIM, NB, bs,
-          _DTYPES[key.dtype])
+    row = H * HEAD_DIM  # a single row may carry any stride
+    _call("store_kvcache_q4", dev, lib().b200_store_kvcache_q4, key.data_ptr(), ks[0] if N > 1 else row,
+          value.data_ptr(), vs[0] if N > 1 else row, k_cache.data_ptr(), v_cache.data_ptr(), slot_mapping.data_ptr(),
+          N, H, HEAD_DIM, cs[0], cs[2], _DTYPES[key.dtype])
 
 
-def _out_rows(out, n, k_cache, dtype):
-    """The (key, value) rows a reader writes."""
-    H = k_cache.size(1)
+def _out_rows(out, n, k_cache, cs, dtype):
+    """The (key, value) rows a reader writes, and their token strides."""
+    H = cs[1]
+    row = H * HEAD_DIM
     if out is None:
-        _refuse_type(dtype, HEAD_DIM)
-        return k_cache.new_empty((n, H, HEAD_DIM), dtype=dtype), k_cache.new_empty((n, H, HEAD_DIM), dtype=dtype)
+        shape = (n, H, HEAD_DIM)
+        return k_cache.new_empty(shape, dtype=dtype), k_cache.new_empty(shape, dtype=dtype), row, row
     key, value = out
-    if not _rows_ok(key, value):
+    shape, ks, vs = key.shape, key.stride(), value.stride()
+    if not _rows_ok(key, value, shape, ks, vs):
         _explain_rows(key, value)
-    assert key.size(0) == n and key.size(1) == H and key.dtype == dtype, \
+    assert shape[0] == n and shape[1] == H and key.dtype is dtype, \
         "out rows do not match the tokens, kv heads and dtype asked for"
-    return key, value
+    if not key.get_device() == value.get_device() == k_cache.get_device():
+        _explain_devices(k_cache, key, value)
+    return key, value, ks[0] if n > 1 else row, vs[0] if n > 1 else row
 
 
 def load_kvcache_q4(k_cache: torch.Tensor, v_cache: torch.Tensor, slot_mapping: torch.Tensor, dtype: torch.dtype,
@@ -149,19 +142,20 @@ def load_kvcache_q4(k_cache: torch.Tensor, v_cache: torch.Tensor, slot_mapping: 
     """Read the records of slot_mapping [N] back: (key, value) rows [N, Hkv, 128] in `dtype`, the type
     the cache was written in.  Slots of -1 or outside the cache read as zeros.  `out` is an optional
     (key, value) pair to write to."""
-    H = k_cache.size(1)
-    if not _cache_ok(k_cache, v_cache, H):
-        _explain_cache(k_cache, v_cache, H)
-    N = slot_mapping.numel()
-    if slot_mapping.dtype != torch.int32 or not slot_mapping.is_contiguous():
+    cs = k_cache.shape
+    if dtype not in _DTYPES:
+        _refuse_type(dtype, HEAD_DIM)
+    if not _cache_ok(k_cache, v_cache, cs):
+        _explain_cache(k_cache, v_cache, cs[1] if len(cs) == 4 else 0)
+    if slot_mapping.dtype is not _I32 or not slot_mapping.is_contiguous():
         _explain_ints("slot_mapping", slot_mapping)
-    key, value = _out_rows(out, N, k_cache, dtype)
     dev = k_cache.get_device()
-    if not _same_device(dev, v_cache, slot_mapping, key, value):
-        _explain_devices(k_cache, v_cache, slot_mapping, key, value)
-    NB, _, bs, _ = k_cache.shape
-    _call("load_kvcache_q4", dev, lib().b200_load_kvcache_q4, key.data_ptr(), _token_stride(key), value.data_ptr(),
-          _token_stride(value), k_cache.data_ptr(), v_cache.data_ptr(), slot_mapping.data_ptr(), N, H, HEAD_DIM, NB, bs,
+    if not (dev >= 0 and v_cache.get_device() == dev and slot_mapping.get_device() == dev):
+        _explain_devices(k_cache, v_cache, slot_mapping)
+    N = slot_mapping.numel()
+    key, value, k_row, v_row = _out_rows(out, N, k_cache, cs, dtype)
+    _call("load_kvcache_q4", dev, lib().b200_load_kvcache_q4, key.data_ptr(), k_row, value.data_ptr(), v_row,
+          k_cache.data_ptr(), v_cache.data_ptr(), slot_mapping.data_ptr(), N, cs[1], HEAD_DIM, cs[0], cs[2],
           _DTYPES[dtype])
     return key, value
 
@@ -177,24 +171,27 @@ def gather_kvcache_q4(k_cache: torch.Tensor, v_cache: torch.Tensor, cu_seqlens: 
     behind the last sequence are left as they were); None reads cu_seqlens[-1] on the host,
     which synchronises.  Tokens of a page outside the cache read as zeros.
     """
-    H = k_cache.size(1)
-    if not _cache_ok(k_cache, v_cache, H):
-        _explain_cache(k_cache, v_cache, H)
+    cs = k_cache.shape
+    if dtype not in _DTYPES:
+        _refuse_type(dtype, HEAD_DIM)
+    if not _cache_ok(k_cache, v_cache, cs):
+        _explain_cache(k_cache, v_cache, cs[1] if len(cs) == 4 else 0)
     S = cu_seqlens.numel() - 1
-    if cu_seqlens.dtype != torch.int32 or S < 0 or not cu_seqlens.is_contiguous():
+    if cu_seqlens.dtype is not _I32 or S < 0 or not cu_seqlens.is_contiguous():
         _explain_ints("cu_seqlens", cu_seqlens)
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.stride(1) != 1 or block_table.size(0) < S:
+    bt = block_table.shape
+    if block_table.dtype is not _I32 or len(bt) != 2 or bt[0] < S or block_table.stride(1) != 1:
         _explain_ints("block_table (a row per sequence)", block_table)
-    n = int(cu_seqlens[-1]) if total_tokens is None else int(total_tokens)
-    assert n >= 0, f"total_tokens {n} < 0"
-    key, value = _out_rows(out, n, k_cache, dtype)
     dev = k_cache.get_device()
-    if not _same_device(dev, v_cache, cu_seqlens, block_table, key, value):
-        _explain_devices(k_cache, v_cache, cu_seqlens, block_table, key, value)
-    NB, _, bs, _ = k_cache.shape
-    _call("gather_kvcache_q4", dev, lib().b200_gather_kvcache_q4, key.data_ptr(), _token_stride(key), value.data_ptr(),
-          _token_stride(value), k_cache.data_ptr(), v_cache.data_ptr(), cu_seqlens.data_ptr(), block_table.data_ptr(),
-          block_table.stride(0), block_table.size(1), S, n, H, HEAD_DIM, NB, bs, _DTYPES[dtype])
+    if not (dev >= 0 and v_cache.get_device() == dev and cu_seqlens.get_device() == dev
+            and block_table.get_device() == dev):
+        _explain_devices(k_cache, v_cache, cu_seqlens, block_table)
+    n = int(cu_seqlens[-1]) if total_tokens is None else int(total_tokens)
+    assert 0 <= n < 2 ** 31, f"total_tokens {n}"
+    key, value, k_row, v_row = _out_rows(out, n, k_cache, cs, dtype)
+    _call("gather_kvcache_q4", dev, lib().b200_gather_kvcache_q4, key.data_ptr(), k_row, value.data_ptr(), v_row,
+          k_cache.data_ptr(), v_cache.data_ptr(), cu_seqlens.data_ptr(), block_table.data_ptr(), block_table.stride(0),
+          bt[1], S, n, cs[1], HEAD_DIM, cs[0], cs[2], _DTYPES[dtype])
     return key, value
 
 
@@ -265,32 +262,35 @@ def flash_attn_with_kvcache_q4(q, k_cache, v_cache, cache_seqlens=None, block_ta
     once; calls that share it must not overlap (default: one per stream, or per captured call).
     """
     assert cache_seqlens is not None and block_table is not None, "the B200 path reads a paged cache"
-    B, Lq, Hq, D = q.shape
+    shape, qs, cs, bt = q.shape, q.stride(), k_cache.shape, block_table.shape
+    B, Lq, Hq, D = shape
     if not causal and Lq > 1:
         raise NotImplementedError("non-causal multi-query paged attention")
-    NB, Hkv, bs, _ = k_cache.shape
     if out is None:
-        out = q.new_empty((B, Lq, Hq, D))
-    qs = q.stride()
-    q_tok = (qs[0] if B > 1 else Hq * D) if Lq == 1 else qs[1]
+        out = q.new_empty(shape)
     dev = q.get_device()
-    if not (D == HEAD_DIM and q.dtype in _DTYPES and _cache_ok(k_cache, v_cache, Hkv) and Hkv > 0 and Hq % Hkv == 0
+    if not (D == HEAD_DIM and q.dtype in _DTYPES and _cache_ok(k_cache, v_cache, cs) and cs[1] > 0 and Hq % cs[1] == 0
             and qs[3] == 1 and (Hq == 1 or qs[2] == D) and (Lq == 1 or B <= 1 or qs[0] == Lq * qs[1])
-            and cache_seqlens.dtype == torch.int32 and cache_seqlens.numel() == B and cache_seqlens.is_contiguous()
-            and block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.stride(1) == 1
-            and block_table.size(0) >= B and out.shape == q.shape and out.is_contiguous() and out.dtype == q.dtype
-            and _same_device(dev, k_cache, v_cache, cache_seqlens, block_table, out)):
+            and cache_seqlens.dtype is _I32 and cache_seqlens.numel() == B and cache_seqlens.is_contiguous()
+            and block_table.dtype is _I32 and len(bt) == 2 and bt[0] >= B and block_table.stride(1) == 1
+            and out.shape == shape and out.dtype is q.dtype and out.is_contiguous()
+            and dev >= 0 and k_cache.get_device() == dev and v_cache.get_device() == dev
+            and cache_seqlens.get_device() == dev and block_table.get_device() == dev and out.get_device() == dev):
         _explain_attention(q, k_cache, v_cache, cache_seqlens, block_table, causal, out)
+    Hkv = cs[1]
     if workspace is None:
         rows = min(Lq * (Hq // Hkv), 16)
-        if torch._C._cuda_getDevice() == dev:
+        if _current_device() == dev:
             workspace = _workspace(dev, rows)
         else:
             with torch.cuda.device(dev):
                 workspace = _workspace(dev, rows)
-    _call("flash_attn_with_kvcache_q4", dev, lib().b200_paged_attention_q4, out.data_ptr(), q.data_ptr(), q_tok,
-          k_cache.data_ptr(), v_cache.data_ptr(), NB, bs, block_table.data_ptr(), block_table.stride(0),
-          block_table.size(1), cache_seqlens.data_ptr(), B, Lq, Hq, Hkv, D,
+    else:
+        assert workspace.dtype is _U8 and workspace.get_device() == dev and workspace.is_contiguous(), \
+            "the workspace must be contiguous uint8 on q's device"
+    _call("flash_attn_with_kvcache_q4", dev, lib().b200_paged_attention_q4, out.data_ptr(), q.data_ptr(),
+          (qs[0] if B > 1 else Hq * D) if Lq == 1 else qs[1], k_cache.data_ptr(), v_cache.data_ptr(), cs[0], cs[2],
+          block_table.data_ptr(), block_table.stride(0), bt[1], cache_seqlens.data_ptr(), B, Lq, Hq, Hkv, D,
           D ** -0.5 if softmax_scale is None else float(softmax_scale), _DTYPES[q.dtype], workspace.data_ptr(),
           workspace.numel())
     return out

@@ -159,7 +159,8 @@ def test_c_abi_refusals(pkg):
     for fn in (lib.b200_store_kvcache_q4, lib.b200_load_kvcache_q4):
         for kw, rc in [(dict(n=0), 0), (dict(n=-1), ARG), (dict(key=None), ARG), (dict(slots=None), ARG), (dict(d=64), UNS),
                        (dict(dt=2), UNS), (dict(h=0), ARG), (dict(nb=0), ARG), (dict(bs=0), ARG), (dict(nb=1 << 24), ARG),
-                       (dict(n=2, ks=255), ARG), (dict(kc=a + 8), ARG), (dict(key=a + 1), ARG)]:
+                       (dict(n=2, ks=255), ARG), (dict(kc=a + 8), ARG), (dict(key=a + 1), ARG),
+                       (dict(nb=1 << 20, bs=1024, h=4, ks=512, vs=512), UNS), (dict(h=65536), ARG)]:  # 2^32 records
             assert store(fn, **kw) == rc, (kw, lib.b200_last_error())
     ga = dict(key=a, ks=256, v=a, vs=256, kc=a, vc=a, cu=a, bt=a, bts=1, btw=1, s=1, n=1, h=2, d=128, nb=1, bs=128, dt=1,
               st=None)

@@ -561,6 +561,9 @@ def test_caller_owned_workspace(pkg):
     with pytest.raises(pkg.B200Error):
         pkg.flash_attn_with_kvcache_q4(args[0], args[1], args[2], cache_seqlens=args[3], block_table=args[4],
                                        workspace=torch.zeros(need - 4096, dtype=torch.uint8, device="cuda"))
+    for bad in (torch.zeros(need, dtype=torch.uint8), ws.view(torch.int32), torch.zeros(2 * need, dtype=torch.uint8, device="cuda")[::2]):
+        with pytest.raises(AssertionError):  # on the host, of another type, with gaps
+            pkg.flash_attn_with_kvcache_q4(args[0], args[1], args[2], cache_seqlens=args[3], block_table=args[4], workspace=bad)
 
 
 def test_wait_that_runs_out_is_reported(pkg):
