@@ -45,9 +45,10 @@
 // bounded (kWaitLimitNs, or the test limit).
 //
 // What bounds it (512 sequences, 1.17 M tokens, 8 kv heads of 4 rows: 1.50 GB, 228 us at the measured
-// copy rate): 280 us, 163 M warp instructions, the vector pipes; held for a second it reaches the
-// board's power cap and 320 us.  A record costs its share of 280 instructions per 16 tokens, 72 of
-// them masks.
+// copy rate): 273 us, 158 M warp instructions, the vector pipes; held for a second it reaches the
+// board's power cap, 1.74 GHz and 308 to 313 us.  A record costs its share of 270 instructions per
+// 16 tokens, 72 of them masks.  16 consumer warps per SM (104 registers each, taken from their
+// producers) issue more often, spill, and take 272 us; they would cost the short calls 2 us.
 #include <atomic>
 #include <cfloat>
 #include <climits>
@@ -78,8 +79,9 @@ constexpr int kKvBytes = kTile * kRecord;  // keys (or values) of one stage
 constexpr int kStageBytes = 2 * kKvBytes;
 constexpr int kMaxBatch = 2048;
 // What a (sequence, kv head) pair costs beside its tiles, in tiles (decode of 512 sequences / verify of
-// 128: 280 / 134 us with 2, 281 / 142 with 1, 284 / 136 with 3, 289 / 138 with 4).
+// 128: 273 / 131 us with 2, 275 / 138 with 1, 278 / 133 with 3, 282 / 134 with 4).
 constexpr int kPairCost = 2;
+constexpr float kCodeUnit = 1.f / 16777216.f;  // 2^-24, the value of code 1 as an fp16 operand
 constexpr float kLazyMax = 8.f;  // log2 headroom before a row's running maximum is raised
 constexpr float kNone = -1e30f;  // reference of a row that has met no token
 constexpr int kExpMax = 60;      // bound of |E| and of the query rows' exponents
@@ -500,6 +502,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
     const uint32_t word_off = uint32_t(lane & 15) * kRecord + q4::kParams;
     const uint32_t trans_off = uint32_t((lane & 7) + (lane >> 4) * 8) * kRecord + q4::kParams;
     const uint32_t look_off = uint32_t(lane) * kRecord + q4::kParams;
+    // Scores in units of 2^-24, which the minima start as the MMAs' result; fp16 sums of q do not go down to
+    // that unit, and 16 rows would spill (131.5 us against 133.4 for the verify call): there they join last.
+    constexpr bool kMinFirst = BF16 && NT == 1;
     constexpr uint32_t kLo = 0x000f000fu, kHi = 0x00f000f0u;
     if (lane < 2) sm.part[warp][lane].nch = 0;
     __syncwarp();
@@ -568,8 +573,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
                     qf[j][nt][2] = pack2<false>(x[j][4], x[j][5]);
                     qf[j][nt][3] = pack2<false>(x[j][6] * 0.0625f, x[j][7] * 0.0625f);
                 }
-                split2<BF16>(make_float2(0.f, mine), qs[nt][0], qs[nt][1]);
-                const float fm = p.scale_log2 * exp2_int(eq);
+                split2<BF16>(make_float2(0.f, mine * (kMinFirst ? kCodeUnit : 1.f)), qs[nt][0], qs[nt][1]);
+                // Above zero even where that underflows (all scores are 0 then): a masked -inf stays one.
+                const float fm = fmaxf(p.scale_log2 * exp2_int(eq) * (kMinFirst ? 1.f / kCodeUnit : 1.f), 1e-30f);
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     const int rw = 8 * nt + 2 * c + e;
@@ -617,7 +623,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
             constexpr bool EDGE = decltype(edge)::value;
             uint8_t* kb = sm.stages[stage] + (tok_warp + sub) * kRecord;
             uint8_t* vb = kb + kKvBytes;
-            // ---- log2 scores x: codes and minima of S^T = K Q^T ----
+            // ---- scores x (times f_row: log2): codes and minima of S^T = K Q^T ----
             float x[2][NT][4];  // sub-tile of 16: token g (+ 8 for e >= 2), rows 8 nt + 2 c, 2 c + 1
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
@@ -628,6 +634,12 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
                 const uint4 pa4 = *reinterpret_cast<const uint4*>(ks + par_off);
                 const uint4 pb4 = *reinterpret_cast<const uint4*>(ks + par_off + 8 * kRecord);
                 const uint32_t pa[4] = {pa4.x, pa4.y, pa4.z, pa4.w}, pb[4] = {pb4.x, pb4.y, pb4.z, pb4.w};
+                uint32_t a[4];  // word c of the parameters of tokens g, g + 8, g, g + 8
+                if constexpr (kMinFirst) {
+                    ldsm_x4(a[0], a[1], a[2], a[3], smem_u32(ks) + word_off);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) mma_zero<BF16>(x[u][nt], a, qs[nt][0], qs[nt][1]);
+                }
 #pragma unroll
                 for (int j = 0; j < kGroups; ++j) {
                     const uint32_t wa = kw[0][j], wb = kw[1][j], wa8 = wa >> 8, wb8 = wb >> 8;
@@ -642,18 +654,19 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             const float sc = e < 2 ? sa : sb;
-                            x[u][nt][e] = j == 0 ? sc * acc[e] : fmaf(sc, acc[e], x[u][nt][e]);
+                            x[u][nt][e] = !kMinFirst && j == 0 ? sc * acc[e] : fmaf(sc, acc[e], x[u][nt][e]);
                         }
                     }
                 }
-                uint32_t a[4];  // word c of tokens g, g + 8, g, g + 8
-                ldsm_x4(a[0], a[1], a[2], a[3], smem_u32(ks) + word_off);
+                if constexpr (!kMinFirst) {
+                    ldsm_x4(a[0], a[1], a[2], a[3], smem_u32(ks) + word_off);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    float xm[4];
-                    mma_zero<BF16>(xm, a, qs[nt][0], qs[nt][1]);
+                    for (int nt = 0; nt < NT; ++nt) {
+                        float xm[4];
+                        mma_zero<BF16>(xm, a, qs[nt][0], qs[nt][1]);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) x[u][nt][e] = fmaf(x[u][nt][e], 16777216.f, xm[e]) * f_row[nt][e & 1];
+                        for (int e = 0; e < 4; ++e) x[u][nt][e] = fmaf(x[u][nt][e], 1.f / kCodeUnit, xm[e]);
+                    }
                 }
             }
             // ---- masks; references ----
@@ -671,7 +684,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int e = 0; e < 2; ++e)
-                    y_max = fmaxf(y_max, max3f(fmaxf(x[0][nt][e], x[0][nt][2 + e]), x[1][nt][e], x[1][nt][2 + e]) - r_ref[nt][e]);
+                    y_max = fmaxf(y_max, fmaf(max3f(fmaxf(x[0][nt][e], x[0][nt][2 + e]), x[1][nt][e], x[1][nt][2 + e]),
+                                              f_row[nt][e], -r_ref[nt][e]));
             const uint4 look = *reinterpret_cast<const uint4*>(vb + look_off);  // value parameters of token `lane`
             const float reach = reach_of<BF16>(look);
             if (__any_sync(0xffffffffu, y_max > kLazyMax || reach > reach_lim)) {
@@ -694,6 +708,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
                         float tm = max3f(fmaxf(x[0][nt][e], x[0][nt][2 + e]), x[1][nt][e], x[1][nt][2 + e]);
 #pragma unroll
                         for (int sh = 4; sh <= 16; sh <<= 1) tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, sh));
+                        tm *= f_row[nt][e];
                         const float ro = r_ref[nt][e], rn = fmaxf(ro, tm == -INFINITY ? kNone : tm);
                         const float alpha = ro == kNone ? 0.f : fast_exp2(ro - rn), alpha_v = alpha * drop;
                         r_ref[nt][e] = rn;
@@ -736,8 +751,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        const float2 y = make_float2(fast_exp2(x[u][nt][2 * i] - r_ref[nt][0]),
-                                                     fast_exp2(x[u][nt][2 * i + 1] - r_ref[nt][1]));
+                        const float2 y = make_float2(fast_exp2(fmaf(x[u][nt][2 * i], f_row[nt][0], -r_ref[nt][0])),
+                                                     fast_exp2(fmaf(x[u][nt][2 * i + 1], f_row[nt][1], -r_ref[nt][1])));
                         if constexpr (BF16) {
                             pb[nt][i] = transpose8(pack2<false>(y.x, y.y));
                         } else {
