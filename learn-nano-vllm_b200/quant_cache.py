@@ -124,8 +124,8 @@ def _out_rows(out, n, k_cache, cs, dtype):
     H = cs[1]
     row = H * HEAD_DIM
     if out is None:
-        shape = (n, H, HEAD_DIM)
-        return k_cache.new_empty(shape, dtype=dtype), k_cache.new_empty(shape, dtype=dtype), row, row
+        key = k_cache.new_empty((n, H, HEAD_DIM), dtype=dtype)
+        return key, torch.empty_like(key), row, row
     key, value = out
     shape, ks, vs = key.shape, key.stride(), value.stride()
     if not _rows_ok(key, value, shape, ks, vs):
@@ -267,7 +267,7 @@ def flash_attn_with_kvcache_q4(q, k_cache, v_cache, cache_seqlens=None, block_ta
     if not causal and Lq > 1:
         raise NotImplementedError("non-causal multi-query paged attention")
     if out is None:
-        out = q.new_empty(shape)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     dev = q.get_device()
     if not (D == HEAD_DIM and q.dtype in _DTYPES and _cache_ok(k_cache, v_cache, cs) and cs[1] > 0 and Hq % cs[1] == 0
             and qs[3] == 1 and (Hq == 1 or qs[2] == D) and (Lq == 1 or B <= 1 or qs[0] == Lq * qs[1])
