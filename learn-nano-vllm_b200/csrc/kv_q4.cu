@@ -13,6 +13,8 @@
 // whose records are neighbours in a page (160 bytes, five whole sectors).  A block takes a run
 // of tokens and looks up once where their records lie; each of its warps takes rows (a head's
 // keys or values) and walks the token pairs, kFlight of them in flight.
+#include <algorithm>
+
 #include "kv_q4.cuh"
 
 namespace b200 {
@@ -20,8 +22,10 @@ namespace q4 {
 namespace {
 
 constexpr int kWarps = 8;
-constexpr int kMaxTokens = 24;    // tokens of one block
-constexpr int kBlocksPerSm = 4;   // resident (launch bounds)
+constexpr int kMaxTokens = 32;  // of one block
+// Resident blocks per SM (launch bounds) and tokens of a block where many waves run: see shape_of.
+constexpr int kStoreBlocks = 4, kStoreTokens = 24;
+constexpr int kReadBlocks = 5, kReadTokens = 16;
 
 struct Rows {
     char* k;  // key rows (read by store, written by load and gather)
@@ -53,12 +57,14 @@ template <int kFlight, typename LOAD, typename USE>
 __device__ __forceinline__ void for_rows(const Rows& rows, const Cache& cache, const uint32_t* s_rec, int64_t t0, int count,
                                          LOAD load, USE use) {
     const int half = (threadIdx.x >> 4) & 1, l = threadIdx.x & 15, pairs = (count + 1) >> 1;
+#pragma unroll 1  // a block comes by once or twice: more code is more to fetch
     for (int r = blockIdx.y * kWarps + (threadIdx.x >> 5); r < 2 * cache.hkv; r += gridDim.y * kWarps) {
         const bool v = r >= cache.hkv;
         const int h = v ? r - cache.hkv : r;
         const int64_t stride = v ? rows.v_stride : rows.k_stride;
         char* row = (v ? rows.v : rows.k) + (t0 + half) * stride + h * (kD * 2) + 16 * l;
         char* records = (v ? cache.v : cache.k) + int64_t(h) * cache.block_size * kRecord;
+#pragma unroll 1
         for (int p0 = 0; p0 < pairs; p0 += kFlight) {
             uint32_t rec[kFlight];
 #pragma unroll
@@ -74,7 +80,7 @@ __device__ __forceinline__ void for_rows(const Rows& rows, const Cache& cache, c
 }
 
 template <bool BF16, bool VEC, int kFlight>
-__global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm)
+__global__ void __launch_bounds__(kWarps * 32, kStoreBlocks)
     store_kernel(const Rows rows, const Cache cache, const int32_t* __restrict__ slots, int32_t n, int32_t tokens) {
     __shared__ uint32_t s_rec[kMaxTokens];
     const int64_t t0 = int64_t(blockIdx.x) * tokens;
@@ -137,7 +143,7 @@ __device__ __forceinline__ void read_rows(const Rows& rows, const Cache& cache, 
 }
 
 template <bool BF16, bool VEC, int kFlight>
-__global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm)
+__global__ void __launch_bounds__(kWarps * 32, kReadBlocks)
     load_kernel(const Rows rows, const Cache cache, const int32_t* __restrict__ slots, int32_t n, int32_t tokens) {
     __shared__ uint32_t s_rec[kMaxTokens];
     const int64_t t0 = int64_t(blockIdx.x) * tokens;
@@ -155,7 +161,7 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm)
 }
 
 template <bool BF16, bool VEC, int kFlight>
-__global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm)
+__global__ void __launch_bounds__(kWarps * 32, kReadBlocks)
     gather_kernel(const Rows rows, const Cache cache, const int32_t* __restrict__ cu, const int32_t* __restrict__ tables,
                   int64_t bt_stride, int32_t bt_width, int32_t num_seqs, int32_t n, int32_t tokens) {
     __shared__ uint32_t s_rec[kMaxTokens];
@@ -186,22 +192,24 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm)
 
 // Launch shape.  Up to two tokens per resident block: latency, a pair of tokens per block and a row per
 // warp (8 tokens x 8 heads, store and load in a graph: 3.6 us against 5.4 with four pairs in flight).
-// More: whole waves of resident blocks, each of at most kMaxTokens tokens and four pairs per warp in
-// flight.  16,384 tokens x 8 heads, store and load: 40.0 us with whole waves of up to 24 tokens, 40.8
-// with powers of two up to 32; gather of 68.6k tokens: 55.8 against 56.9 us; 6 resident blocks of 40
-// registers lose 2 us on both and win 8 us of 112 on four sequences of 26k.
+// More: four pairs per warp in flight, at least three of them full (2500 tokens, store and load: 8.7 us
+// against 9.5 with two; 1500: 7.2, with four 7.7); one wave of resident blocks while they can hold it
+// (16,384 tokens: 37 us against 38.3 in two waves), else whole waves of shorter blocks (gather of 68.6k tokens:
+// 53.2 us with up to 16 tokens, 55.2 with 24; store and load of 40,000: 86.4 us with 24 tokens in the store's, 89.0
+// with 16).  Reading wants the fifth block of 48 registers (gather of four sequences of 26k: 104.8 us against
+// 111.7), storing loses by it (16,384 tokens: 39.5 us).
 struct Shape {
     int tokens;
     dim3 grid;
     bool small;
 };
 
-Shape shape_of(int32_t n, int32_t hkv) {
-    const int64_t blocks = int64_t(kBlocksPerSm) * device_sm_count();
+Shape shape_of(int32_t n, int32_t hkv, int per_sm, int wave_tokens) {
+    const int64_t blocks = int64_t(per_sm) * device_sm_count();
     Shape s;
     s.small = n <= 2 * blocks;
-    const int64_t waves = (n + kMaxTokens * blocks - 1) / (kMaxTokens * blocks);
-    s.tokens = s.small ? 2 : int((n + waves * blocks - 1) / (waves * blocks) + 1) & ~1;
+    const int64_t waves = n <= kMaxTokens * blocks ? 1 : (n + wave_tokens * blocks - 1) / (wave_tokens * blocks);
+    s.tokens = s.small ? 2 : std::max(6, int((n + waves * blocks - 1) / (waves * blocks) + 1) & ~1);
     s.grid = dim3((unsigned(n) + s.tokens - 1) / s.tokens, s.small ? (2 * hkv + kWarps - 1) / kWarps : 1);
     return s;
 }
@@ -240,9 +248,9 @@ bool vector_rows(const Rows& r) {
         if (shape.small) KERNEL<BF16, VEC, 1><<<shape.grid, kWarps * 32, 0, st>>>(__VA_ARGS__); \
         else KERNEL<BF16, VEC, 4><<<shape.grid, kWarps * 32, 0, st>>>(__VA_ARGS__);           \
     } while (0)
-#define B200_Q4_LAUNCH(KERNEL, n, ...)                                           \
+#define B200_Q4_LAUNCH(KERNEL, PER_SM, n, ...)                                           \
     do {                                                                         \
-        const Shape shape = shape_of(n, num_kv_heads);                           \
+        const Shape shape = shape_of(n, num_kv_heads, PER_SM##Blocks, PER_SM##Tokens);                           \
         cudaStream_t st = static_cast<cudaStream_t>(stream);                     \
         const bool vec = vector_rows(rows);                                      \
         if (dtype == B200_BF16 && vec) B200_Q4_CASE(KERNEL, true, true, __VA_ARGS__, shape.tokens);  \
@@ -273,7 +281,7 @@ extern "C" int32_t b200_store_kvcache_q4(const void* key, int64_t key_stride, co
                     key_stride * 2, value_stride * 2};
     const Cache cache{static_cast<char*>(k_cache), static_cast<char*>(v_cache), num_kv_heads, block_size,
                       int64_t(num_blocks) * block_size};
-    B200_Q4_LAUNCH(store_kernel, num_tokens, rows, cache, slot_mapping, num_tokens);
+    B200_Q4_LAUNCH(store_kernel, kStore, num_tokens, rows, cache, slot_mapping, num_tokens);
     return B200_OK;
 }
 
@@ -293,7 +301,7 @@ extern "C" int32_t b200_load_kvcache_q4(void* key, int64_t key_stride, void* val
     const Rows rows{static_cast<char*>(key), static_cast<char*>(value), key_stride * 2, value_stride * 2};
     const Cache cache{static_cast<char*>(const_cast<void*>(k_cache)), static_cast<char*>(const_cast<void*>(v_cache)),
                       num_kv_heads, block_size, int64_t(num_blocks) * block_size};
-    B200_Q4_LAUNCH(load_kernel, num_tokens, rows, cache, slot_mapping, num_tokens);
+    B200_Q4_LAUNCH(load_kernel, kRead, num_tokens, rows, cache, slot_mapping, num_tokens);
     return B200_OK;
 }
 
@@ -317,7 +325,7 @@ extern "C" int32_t b200_gather_kvcache_q4(void* key, int64_t key_stride, void* v
     const Rows rows{static_cast<char*>(key), static_cast<char*>(value), key_stride * 2, value_stride * 2};
     const Cache cache{static_cast<char*>(const_cast<void*>(k_cache)), static_cast<char*>(const_cast<void*>(v_cache)),
                       num_kv_heads, block_size, int64_t(num_blocks) * block_size};
-    B200_Q4_LAUNCH(gather_kernel, total_tokens, rows, cache, cu_seqlens, block_tables, block_table_stride,
+    B200_Q4_LAUNCH(gather_kernel, kRead, total_tokens, rows, cache, cu_seqlens, block_tables, block_table_stride,
                    block_table_width, num_seqs, total_tokens);
     return B200_OK;
 }

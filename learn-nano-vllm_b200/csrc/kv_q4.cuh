@@ -107,22 +107,32 @@ __device__ __forceinline__ uint32_t quantise8(const uint32_t (&x)[4], uint32_t& 
     return finite ? word : 0u;
 }
 
-// The eight values of a word of codes, rounded to the model's type (four packed pairs).
+template <bool BF16>
+__device__ __forceinline__ uint32_t fma2_16(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t d;
+    if constexpr (BF16) asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+    else asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+    return d;
+}
+
+// The eight values s n + m of a word of codes in the model's type (four packed pairs), each rounded once.
+// A code in the low mantissa bits of 128 (bf16) or 1024 (fp16) is that number plus n, exactly; taking it
+// off again in 16 bits is exact too.  fp16 has room for the next nibble, 16 n, as it stands.  (Gather of four
+// sequences of 26k tokens: 109.6 us against 111.9 with the codes taken to fp32.)
 template <bool BF16>
 __device__ __forceinline__ uint4 dequantise8(uint32_t word, uint32_t params) {
-    const float s = lo_f<BF16>(params), m = hi_f<BF16>(params);
-    const uint32_t odd = word >> 16;
+    const uint32_t s = __byte_perm(params, 0, 0x1010), m = __byte_perm(params, 0, 0x3232);
     uint32_t y[4];
-    float si = s;
 #pragma unroll
-    for (int i = 0; i < 4; ++i, si *= 0.0625f) {
-        // 2^23 + 16^i code is exact in fp32, and so are s / 16^i and the product: one rounding in the
-        // sum, one to 16 bits.
-        const float2 c = fsub2(make_float2(__uint_as_float(0x4b000000u | (word & (15u << (4 * i)))),
-                                           __uint_as_float(0x4b000000u | (odd & (15u << (4 * i))))),
-                               make_float2(8388608.f, 8388608.f));
-        const float2 v = ffma2(c, make_float2(si, si), make_float2(m, m));
-        y[i] = pack2<BF16>(v.x, v.y);
+    for (int i = 0; i < 4; ++i) {
+        uint32_t n;
+        if constexpr (BF16)
+            n = fma2_16<BF16>(((word >> (4 * i)) & 0x000f000fu) | 0x43004300u, 0x3f803f80u, 0xc300c300u);
+        else if (i & 1)
+            n = fma2_16<BF16>(((word >> (4 * i - 4)) & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, 0xd400d400u);
+        else
+            n = fma2_16<BF16>(((word >> (4 * i)) & 0x000f000fu) | 0x64006400u, 0x3c003c00u, 0xe400e400u);
+        y[i] = fma2_16<BF16>(n, s, m);
     }
     return make_uint4(y[0], y[1], y[2], y[3]);
 }

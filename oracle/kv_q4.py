@@ -14,10 +14,13 @@ def float_bits(x, bf16):
     """uint16 patterns of float64 values rounded to bf16 / fp16 (nearest even); NaN -> 0x7fff."""
     x = np.asarray(x, np.float64)
     if bf16:
-        # fp32 holds every bf16 midpoint exactly; a value that rounds onto one in fp32 but is not one
-        # itself would need 16 more bits than a quotient of 16-bit operands by 15 can differ by.
-        with np.errstate(over="ignore"):
-            u = x.astype(np.float32).view(np.uint32).astype(np.uint64)
+        # Through fp32 rounded to odd (an inexact value ends in a one), which no second rounding can tell
+        # from the value itself.
+        with np.errstate(over="ignore", invalid="ignore"):
+            f = x.astype(np.float32)
+            even = (f.view(np.uint32) & 1 == 0) & (f != x) & np.isfinite(f)
+            f = np.where(even, np.nextafter(f, np.where(x > f, np.float32(np.inf), np.float32(-np.inf))), f)
+            u = f.view(np.uint32).astype(np.uint64)
         r = ((u + 0x7fff + ((u >> 16) & 1)) >> 16).astype(np.uint16)
     else:
         with np.errstate(over="ignore"):

@@ -36,9 +36,9 @@ def oracle_store(cache, x, slots):
 
 
 def oracle_rows(rec, dtype):
-    """Rows in the model's type: one fp32 rounding of the sum, one to 16 bits (as the kernels do)."""
+    """Rows in the model's type: the 64-bit values, rounded once."""
     bf = dtype == BF16
-    v = kv_q4.values(rec, bf).astype(np.float32)
+    v = kv_q4.bits_float(kv_q4.float_bits(kv_q4.values(rec, bf), bf), bf)
     return torch.from_numpy(v).to(dtype)
 
 
@@ -118,6 +118,26 @@ def test_quantise_borders(pkg, dtype):
     ko, vo = pkg.load_kvcache_q4(kc, vc, slots, dtype)
     assert same(ko, oracle_rows(want, dtype)) and same(vo, ko)
     assert torch.isnan(ko[6, 0, 32:64]).all() and torch.isfinite(ko[6, 0, :32]).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_rows_are_rounded_once(pkg, dtype):
+    """A code times its scale half way between two 16-bit numbers, and a minimum far below the last bit of
+    the product: 3 s = 3 + 4.5 units lies above the middle by the minimum, which fp32 would drop."""
+    unit = 2.0 ** -7 if dtype == BF16 else 2.0 ** -10
+    tiny = 2.0 ** -40 if dtype == BF16 else 2.0 ** -24
+    s = 1 + 3 * unit
+    x = torch.full((1, 1, 128), tiny, dtype=torch.float64)
+    x[..., 1::32], x[..., 2::32] = 15 * s, 3 * s
+    x = x.to(dtype).cuda()
+    kc, vc = empty_cache(1, 1, 128), empty_cache(1, 1, 128)
+    slot = torch.zeros(1, dtype=torch.int32, device="cuda")
+    pkg.store_kvcache_q4(x, x, kc, vc, slot)
+    rec = oracle_records(x)
+    codes, scales, _ = kv_q4.unpack(rec, dtype == BF16)
+    assert (scales == s).all() and (codes[..., 2] == 3).all() and (codes[..., 1] == 15).all()
+    ko, _ = pkg.load_kvcache_q4(kc, vc, slot, dtype)
+    assert (ko[..., 2::32].double() == 3 + 10 * unit).all() and same(ko, oracle_rows(rec, dtype))
 
 
 def test_rows_of_any_alignment(pkg):
