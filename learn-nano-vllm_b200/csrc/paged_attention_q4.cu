@@ -129,12 +129,14 @@ struct Cfg {
 int grid_ctas(int rows) { return device_sm_count() * (rows > 8 ? Cfg<2>::kCtas : Cfg<1>::kCtas); }
 
 // Workspace: control words ([2] error word), counters of the CTAs' last items (one per consumer
-// warp), two partial results per CTA and, once per consumer warp, their log-sum-exps.
+// warp; the larger grid's, so that calls of any number of rows can take turns on one workspace), two
+// partial results per CTA and, once per consumer warp, their log-sum-exps.
 constexpr size_t kCtrlBytes = 256;
-size_t fixed_bytes(int ctas) { return kCtrlBytes + ((size_t(ctas) * kWarps * 4 + 255) & ~size_t(255)); }
+size_t fixed_bytes() { return kCtrlBytes + ((size_t(grid_ctas(1)) * kWarps * 4 + 255) & ~size_t(255)); }
+static_assert(Cfg<1>::kCtas >= Cfg<2>::kCtas, "fixed_bytes() is the larger grid's");
 size_t workspace_bytes(int rows) {
     const int ctas = grid_ctas(rows);
-    return (fixed_bytes(ctas) + size_t(2) * ctas * rows * (kD + kWarps) * 4 + 255) & ~size_t(255);
+    return (fixed_bytes() + size_t(2) * ctas * rows * (kD + kWarps) * 4 + 255) & ~size_t(255);
 }
 
 constexpr int kRowPad = kD + 1;  // floats: the lanes of a fragment write 32 different banks
@@ -1034,7 +1036,7 @@ extern "C" int32_t b200_paged_attention_q4(void* out, const void* q, int64_t q_s
     char* ws = static_cast<char*>(workspace);
     prm.error = reinterpret_cast<int32_t*>(ws) + 2;
     prm.counters = reinterpret_cast<int32_t*>(ws + kCtrlBytes);
-    prm.part_o = reinterpret_cast<float*>(ws + fixed_bytes(ctas));
+    prm.part_o = reinterpret_cast<float*>(ws + fixed_bytes());
     prm.part_lse = prm.part_o + size_t(2) * ctas * rows * kD;
     take_test_hook(&prm.wait_ns, &prm.idle_producer);
 

@@ -586,6 +586,22 @@ def test_caller_owned_workspace(pkg):
             pkg.flash_attn_with_kvcache_q4(args[0], args[1], args[2], cache_seqlens=args[3], block_table=args[4], workspace=bad)
 
 
+def test_workspace_serves_every_number_of_rows(pkg):
+    """Decode and verify calls in turn on one workspace (the stream's, and a caller's own): the counters of one
+    do not lie where another keeps its partial results."""
+    decode = make([60000, 3000, 20000], 32, 8, seed=40)
+    verify = make([50000, 2000, 30000], 16, 8, lq=5, seed=41)
+    ws = torch.zeros(max(pkg.q4_workspace_size(1, 4), pkg.q4_workspace_size(5, 2)), dtype=torch.uint8, device="cuda")
+    first = check(pkg, *decode, what="decode"), check(pkg, *verify, what="verify")
+    for kw in (dict(), dict(workspace=ws)):
+        for _ in range(2):
+            for args, want in zip((decode, verify), first):
+                got = pkg.flash_attn_with_kvcache_q4(args[0], args[1], args[2], cache_seqlens=args[3], block_table=args[4],
+                                                     out=torch.full_like(args[0], 7.0), **kw)
+                assert torch.equal(got, want)
+    assert pkg.workspace_error(ws) == 0
+
+
 def test_wait_that_runs_out_is_reported(pkg):
     """The producer issues nothing (test hook): the call returns with error bit 1, the next one is normal."""
     args = make([300, 1100], 16, 8, seed=31)
