@@ -589,8 +589,8 @@ def test_caller_owned_workspace(pkg):
 def test_workspace_serves_every_number_of_rows(pkg):
     """Decode and verify calls in turn on one workspace (the stream's, and a caller's own): the counters of one
     do not lie where another keeps its partial results."""
-    decode = make([60000, 3000, 20000], 32, 8, seed=40)
-    verify = make([50000, 2000, 30000], 16, 8, lq=5, seed=41)
+    decode = make([9000, 500, 4000], 32, 8, seed=40)
+    verify = make([8000, 300, 5000], 16, 8, lq=5, seed=41)
     ws = torch.zeros(max(pkg.q4_workspace_size(1, 4), pkg.q4_workspace_size(5, 2)), dtype=torch.uint8, device="cuda")
     first = check(pkg, *decode, what="decode"), check(pkg, *verify, what="verify")
     for kw in (dict(), dict(workspace=ws)):
