@@ -107,7 +107,7 @@ def store_kvcache_q4(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tens
     N, H, _ = shape
     if not (_cache_ok(k_cache, v_cache, cs) and cs[1] == H):
         _explain_cache(k_cache, v_cache, H)
-    if slot_mapping.dtype is not _I32 or slot_mapping.numel() != N or not slot_mapping.is_contiguous():
+    if slot_mapping.dtype is not _I32 or slot_mapping.numel() != N or N >= 2 ** 31 or not slot_mapping.is_contiguous():
         _explain_ints("slot_mapping", slot_mapping)
     dev = key.get_device()
     if not (dev >= 0 and value.get_device() == dev and k_cache.get_device() == dev and v_cache.get_device() == dev
@@ -147,12 +147,12 @@ def load_kvcache_q4(k_cache: torch.Tensor, v_cache: torch.Tensor, slot_mapping: 
         _refuse_type(dtype, HEAD_DIM)
     if not _cache_ok(k_cache, v_cache, cs):
         _explain_cache(k_cache, v_cache, cs[1] if len(cs) == 4 else 0)
-    if slot_mapping.dtype is not _I32 or not slot_mapping.is_contiguous():
+    N = slot_mapping.numel()
+    if slot_mapping.dtype is not _I32 or N >= 2 ** 31 or not slot_mapping.is_contiguous():
         _explain_ints("slot_mapping", slot_mapping)
     dev = k_cache.get_device()
     if not (dev >= 0 and v_cache.get_device() == dev and slot_mapping.get_device() == dev):
         _explain_devices(k_cache, v_cache, slot_mapping)
-    N = slot_mapping.numel()
     key, value, k_row, v_row = _out_rows(out, N, k_cache, cs, dtype)
     _call("load_kvcache_q4", dev, lib().b200_load_kvcache_q4, key.data_ptr(), k_row, value.data_ptr(), v_row,
           k_cache.data_ptr(), v_cache.data_ptr(), slot_mapping.data_ptr(), N, cs[1], HEAD_DIM, cs[0], cs[2],
