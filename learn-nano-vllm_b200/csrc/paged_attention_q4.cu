@@ -35,7 +35,7 @@
 // as many CTAs as its share of the work.  Every CTA plans its run from context_lens (no host sync:
 // the call can be captured).  A CTA leaves at most two partial results, its first and its last; the
 // warp that finishes the last chunk of a split pair (one counter per consumer warp) merges its
-// share of the outputs.
+// share of the outputs, many chunks in groups first.
 //
 // CTA.  Four consumer warps and a producer warp; three CTAs per SM up to 8 query rows (15 warps
 // leave 128 registers a thread), two for up to 16 (168).  A stage is 128 records of keys and 128 of
@@ -267,18 +267,36 @@ __device__ __forceinline__ int64_t out_row(const Params& p, int b, int h, int r)
     return ((int64_t(b) * p.lq + j) * p.hq + h * p.group + (r - j * p.group)) * kD;
 }
 
-// Merges the chunks of a split pair for this warp's share of each pass of kPassRows rows, kFlight chunks'
-// loads in flight; called by the warp that finished the last chunk.  (52 chunks of one 32k sequence, the
-// whole call: 22.8 us with 8 in flight, 22.0 with 16; 3 chunks of a short one: 9.3 with 4, 10.3 with 16.)
+// log2 of a sum of weights den * 2^m; a NaN is handed on as an infinite weight: the merge's maximum skips NaN.
+__device__ __forceinline__ float log_weight(float m, float den) {
+    return den == 0.f ? -INFINITY : (den <= FLT_MAX ? m + fast_log2(den) : INFINITY);
+}
+
+// Up to 40 chunks of a split pair are merged at once; more in groups of group_of(nch) and what is left, whose
+// results, at most 16, are merged in turn.  (The whole call, at once / in groups: one sequence of 200k and
+// one kv head, 444 chunks, 43.5 / 20.6 us; 32k and two heads 21.9 / 14.7; 32k and eight, 52 chunks, 20.8 / 20.2; 8k and
+// eight, 33 chunks, 13.9 / 14.2.)
+__device__ __forceinline__ int group_of(int nch) { return nch <= 40 ? nch : max(8, (nch + 15) / 16); }
+
+// Partial results that are merged: number u lies in slot `head` (u = 0) or base + step * u.  The result goes to
+// the outputs of hd's pair (to < 0) or to slot `to`.
+struct Merge {
+    int64_t head, base, to;
+    int step, n;
+};
+
+// Merges this warp's share of each pass of kPassRows rows, kFlight chunks' loads in flight; called by the warp
+// that finished the last of them.  (3 chunks of a short sequence, the whole call: 9.3 us with 4 in flight, 10.3
+// with 16.)
 template <bool BF16, int NT, int kFlight>
-__device__ __forceinline__ void merge_share(const Params& p, const Header& hd, int warp, int lane) {
+__device__ __forceinline__ void merge_share(const Params& p, const Header& hd, const Merge& mg, int warp, int lane) {
     using C = Cfg<NT>;
     for (int r0 = 0; r0 < p.rows; r0 += C::kPassRows) {
         const int share = min(C::kPassRows, p.rows - r0) * (kD / kWarps);
         for (int i = 4 * lane; i < share; i += 128) {
             const int e = r0 * kD + warp * share + i, r = e >> 7, d = e & (kD - 1);
             float m = -INFINITY, den = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-            for (int c0 = 0; c0 < hd.nch; c0 += kFlight) {
+            for (int c0 = 0; c0 < mg.n; c0 += kFlight) {
                 float lse[kFlight];
                 float4 x[kFlight];
                 float mx = m;
@@ -286,8 +304,8 @@ __device__ __forceinline__ void merge_share(const Params& p, const Header& hd, i
                 for (int u = 0; u < kFlight; ++u) {
                     lse[u] = -INFINITY;
                     x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (c0 + u < hd.nch) {
-                        const int64_t slot = 2 * int64_t(hd.first + c0 + u) + (c0 + u == 0 ? 1 : 0);
+                    if (c0 + u < mg.n) {
+                        const int64_t slot = c0 + u == 0 ? mg.head : mg.base + mg.step * (c0 + u);
                         lse[u] = __ldcg(p.part_lse + (slot * kWarps + warp) * p.rows + r);
                         x[u] = __ldcg(reinterpret_cast<const float4*>(p.part_o + (slot * p.rows + r) * kD + d));
                     }
@@ -311,8 +329,14 @@ __device__ __forceinline__ void merge_share(const Params& p, const Header& hd, i
                 m = mx;
             }
             const float inv = den == 0.f ? 0.f : __fdividef(1.f, den);
-            *reinterpret_cast<uint2*>(p.out + out_row(p, hd.b, hd.h, r) + d) =
-                make_uint2(pack2<BF16>(acc[0] * inv, acc[1] * inv), pack2<BF16>(acc[2] * inv, acc[3] * inv));
+            if (mg.to < 0) {
+                *reinterpret_cast<uint2*>(p.out + out_row(p, hd.b, hd.h, r) + d) =
+                    make_uint2(pack2<BF16>(acc[0] * inv, acc[1] * inv), pack2<BF16>(acc[2] * inv, acc[3] * inv));
+            } else {
+                *reinterpret_cast<float4*>(p.part_o + (mg.to * p.rows + r) * kD + d) =
+                    make_float4(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
+                if (i == 0 || d == 0) p.part_lse[(mg.to * kWarps + warp) * p.rows + r] = log_weight(m, den);
+            }
         }
     }
 }
@@ -902,9 +926,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
                 float den = 0.f;
 #pragma unroll
                 for (int w = 0; w < kWarps; ++w) den = fmaf(sm.cl[w][lane], fast_exp2(sm.cm[w][lane] - M), den);
-                // A NaN sum is handed on as an infinite weight: the merge's maximum skips NaN.
-                p.part_lse[(slot * kWarps + warp) * p.rows + r0 + lane] =
-                    den == 0.f ? -INFINITY : (den <= FLT_MAX ? M + fast_log2(den) : INFINITY);
+                p.part_lse[(slot * kWarps + warp) * p.rows + r0 + lane] = log_weight(M, den);
             }
             mbar_arrive(&sm.cbar);
             reading = true;
@@ -919,24 +941,40 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
 
     // The run's partial items (its first and its last), after the loop so that the merge's registers are
     // not held beside it: publish this warp's share of each (one release fence per warp, cumulative over the
-    // warp barrier), then count it; the last chunk's warp of this number merges the share.
-    __syncwarp();
+    // warp barrier), then count it; the last chunk's warp of this number merges the share.  Groups are
+    // counted and merged in what belongs to their second chunk's CTA, which has no other item.
+    auto arrive_last = [&](int cta, int n) {
+        __syncwarp();
+        int last = 0;
+        if (lane == 0) {
+            int32_t* counter = &p.counters[cta * kWarps + warp];
+            __threadfence();
+            last = atomicAdd(counter, 1) == n - 1;
+            if (last) {
+                __threadfence();
+                *counter = 0;
+            }
+        }
+        return __shfl_sync(0xffffffffu, last, 0);
+    };
 #pragma unroll 1
     for (int i = 0; i < 2; ++i) {
         const Header hd = sm.part[warp][i];
         if (hd.nch == 0) continue;
-        int last = 0;
-        int32_t* counter = &p.counters[hd.first * kWarps + warp];
-        if (lane == 0) {
-            __threadfence();
-            last = atomicAdd(counter, 1) == hd.nch - 1;
-            if (last) __threadfence();
+        Merge mg{2 * int64_t(hd.first) + 1, 2 * int64_t(hd.first), -1, 2, hd.nch};
+        const int size = group_of(hd.nch), groups = hd.nch / size;
+        if (groups > 1) {
+            const int grp = min((int(blockIdx.x) - hd.first) / size, groups - 1), c0 = grp * size, cta = hd.first + c0 + 1;
+            const int n = grp == groups - 1 ? hd.nch - c0 : size;
+            if (!arrive_last(cta, n)) continue;
+            const int64_t at = 2 * int64_t(hd.first + c0);
+            merge_share<BF16, NT, 16>(p, hd, Merge{at + (grp == 0), at, 2 * int64_t(cta) + 1, 2, n}, warp, lane);
+            const int64_t to = 2 * int64_t(hd.first + 1) + 1;
+            mg = Merge{to, to, -1, 2 * size, groups};
         }
-        if (__shfl_sync(0xffffffffu, last, 0)) {
-            if (hd.nch <= 4) merge_share<BF16, NT, 4>(p, hd, warp, lane);
-            else merge_share<BF16, NT, 16>(p, hd, warp, lane);
-            if (lane == 0) *counter = 0;
-        }
+        if (!arrive_last(hd.first, mg.n)) continue;
+        if (mg.n <= 4) merge_share<BF16, NT, 4>(p, hd, mg, warp, lane);
+        else merge_share<BF16, NT, 16>(p, hd, mg, warp, lane);
     }
 }
 

@@ -586,6 +586,34 @@ def test_caller_owned_workspace(pkg):
             pkg.flash_attn_with_kvcache_q4(args[0], args[1], args[2], cache_seqlens=args[3], block_table=args[4], workspace=bad)
 
 
+@pytest.mark.parametrize("ctx,hq,hkv,lq,dtype", [([57000], 4, 1, 1, BF16), ([57000], 16, 1, 1, F16), ([33000, 100, 9000], 4, 2, 5, BF16),
+                                                 ([28000, 28000], 2, 2, 1, F16), ([9000, 1, 16500], 8, 1, 1, BF16)])
+def test_many_chunks(pkg, ctx, hq, hkv, lq, dtype):
+    """Sequences over so many CTAs that their partial results are merged in groups first: right, the same
+    each time, and on a workspace that is left re-armed."""
+    args = make(ctx, hq, hkv, lq=lq, dtype=dtype, seed=sum(ctx))
+    ws = torch.zeros(pkg.q4_workspace_size(lq, hq // hkv), dtype=torch.uint8, device="cuda")
+    a = check(pkg, *args, what=f"{ctx} {hq}/{hkv}", workspace=ws)
+    assert int(ws[:7424].view(torch.int32).abs().sum()) == 0
+    for _ in range(3):
+        assert torch.equal(a, pkg.flash_attn_with_kvcache_q4(args[0], args[1], args[2], cache_seqlens=args[3],
+                                                             block_table=args[4], out=torch.zeros_like(a), workspace=ws))
+
+
+def test_poison_survives_grouped_merges(pkg):
+    """A NaN value among 57,000 makes its group of 32 dimensions NaN for the rows that see it, and nothing else."""
+    q, kc, vc, cl, bt = make([57000], 2, 1, lq=3, seed=42)
+    want = pkg.flash_attn_with_kvcache_q4(q, kc, vc, cache_seqlens=cl, block_table=bt, softmax_scale=0.09)
+    for token, rows_hit in ((20001, 3), (56998, 2), (56999, 1)):
+        bad = vc.clone()
+        bad[int(bt[0, token // 256]), 0, token % 256, 64 + 4 * 2:64 + 4 * 3] = 0xff  # group 2: s = m = NaN
+        got = pkg.flash_attn_with_kvcache_q4(q, kc, bad, cache_seqlens=cl, block_table=bt, softmax_scale=0.09)
+        hit = torch.zeros_like(got, dtype=torch.bool)
+        hit[:, 3 - rows_hit:, :, 64:96] = True
+        assert torch.equal(torch.isnan(got), hit)
+        assert (got[~hit].float() - want[~hit].float()).abs().max() <= 2 ** -7 * want.float().abs().max()
+
+
 def test_workspace_serves_every_number_of_rows(pkg):
     """Decode and verify calls in turn on one workspace (the stream's, and a caller's own): the counters of one
     do not lie where another keeps its partial results."""
