@@ -156,6 +156,7 @@ struct Smem {
     uint64_t empty[kStages];
     uint64_t cbar;
     int32_t off[kConsumers / 2];  // length before each entry of 2 ceil(batch / 128) sequences
+    int32_t lens[kMaxBatch];      // context lengths in [0, cap]
     int32_t red[kWarps];
     int32_t err;
 };
@@ -256,7 +257,18 @@ __device__ __forceinline__ bool consumer_wait(uint64_t* bar, uint32_t& phase, ui
     return __all_sync(0xffffffffu, ok);
 }
 
-__device__ __forceinline__ int tiles_of(int ctx, int cap) { return (min(max(ctx, 0), cap) + kTile - 1) / kTile; }
+__device__ __forceinline__ int tiles_of(int ctx) { return (ctx + kTile - 1) / kTile; }
+
+__device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
+    asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
+
+// Counts one arrival: what the warp wrote before is visible to whoever counts after it, and the other way round.
+__device__ __forceinline__ int atomic_inc_acq_rel(int32_t* at) {
+    int old;
+    asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(old) : "l"(at) : "memory");
+    return old;
+}
 
 // Length of a pair of nt tiles on the line that is cut into runs: its tiles, then kPairCost.
 __device__ __forceinline__ int span_of(int nt) { return nt > 0 ? nt + kPairCost : 0; }
@@ -366,7 +378,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
     {
         int mine = 0, before = 0;
         if (warp < kWarps) {
-            for (int b = tid * run; b < min((tid + 1) * run, p.batch); ++b) mine += span_of(tiles_of(p.context_lens[b], cap));
+            for (int b = tid * run; b < min((tid + 1) * run, p.batch); ++b) {
+                const int ctx = min(max(p.context_lens[b], 0), cap);
+                sm.lens[b] = ctx;
+                mine += span_of(tiles_of(ctx));
+            }
             before = mine;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -388,70 +404,50 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
     const int quota = max(1, (total + int(gridDim.x) - 1) / int(gridDim.x));
     const int begin = int(min(int64_t(blockIdx.x) * quota, int64_t(total))), end = min(begin + quota, total);
 
-    // Rows without a cached token (CUDA-graph padding) have no tiles and get a zero output.
-    const int64_t row_vec = int64_t(p.lq) * p.hq * kD / 8;  // uint4 per batch row
-    for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
-        if (p.context_lens[b] <= 0) {
-            uint4* o = reinterpret_cast<uint4*>(p.out) + b * row_vec;
-            for (int64_t i = tid; i < row_vec; i += kThreads) o[i] = make_uint4(0, 0, 0, 0);
-        }
-    }
-    if (begin >= end) return;
-
     if (warp == kWarps) {
         // ------------------------------------------------------------ producer
+        if (begin >= end) return;
+        // First pair of the run: its entry of off[] (the last that begins at or before it), then along the entry.
+        static_assert(kConsumers / 2 == 64, "two entries per lane");
+        const int entry = __popc(__ballot_sync(0xffffffffu, sm.off[lane] * p.hkv <= begin)) +
+                          __popc(__ballot_sync(0xffffffffu, sm.off[32 + lane] * p.hkv <= begin)) - 1;
         if (lane == 0 && !p.idle_producer) {
             const uint64_t pol = l2_policy_evict_first();
             const uint32_t q_bytes = uint32_t(p.group) * kD * 2;  // one query token's rows of this kv head
-            // First pair of the run: its entry of off[] by binary search, then along the entry.
-            int lo = 0, hi = kConsumers / 2;
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1;
-                if (sm.off[mid] * p.hkv <= begin) lo = mid; else hi = mid;
-            }
-            int b = 2 * lo * run, at = sm.off[lo] * p.hkv;  // `at`: where the current pair begins
-            int ctx = min(p.context_lens[b], cap), nt = tiles_of(ctx, cap);
+            int b = 2 * entry * run, at = sm.off[entry] * p.hkv;  // `at`: where the current pair begins
+            int ctx = sm.lens[b], nt = tiles_of(ctx);
             while (at + span_of(nt) * p.hkv <= begin) {
                 at += span_of(nt) * p.hkv;
-                ctx = min(p.context_lens[++b], cap);
-                nt = tiles_of(ctx, cap);
+                ctx = sm.lens[++b];
+                nt = tiles_of(ctx);
             }
             int h = (begin - at) / span_of(nt);
             at += h * span_of(nt);
             int t = begin - at;
-            // The next sequence's length and the next tile's page are loaded one step ahead.
-            int ctx_next = p.context_lens[min(b + 1, p.batch - 1)];
             const int64_t head_bytes = int64_t(p.block_size) * kRecord, page_bytes = p.hkv * head_bytes;
             const int32_t* table = p.block_tables + b * p.bt_stride;
             int page = 0, off = 0;  // of tile t
-            Header item{b, h, 0, 0};
             // The first tile of the next pair that has one, if it lies in this run.
             auto next_pair = [&] {
                 t = page = off = 0;
                 at += span_of(nt);
                 if (at >= end) return;
-                if (++item.h == p.hkv) {
-                    item.h = 0;
+                if (++h == p.hkv) {
+                    h = 0;
                     do {
-                        ++item.b;
-                        ctx = min(ctx_next, cap);
-                        nt = tiles_of(ctx, cap);
-                        ctx_next = p.context_lens[min(item.b + 1, p.batch - 1)];
+                        ctx = sm.lens[++b];
+                        nt = tiles_of(ctx);
                     } while (nt == 0);
-                    table = p.block_tables + item.b * p.bt_stride;
+                    table = p.block_tables + b * p.bt_stride;
                 }
-                item.first = at / quota;
-                item.nch = (at + nt - 1) / quota - item.first + 1;
             };
-            if (t < nt) {
+            if (t >= nt) {
+                next_pair();
+            } else if (t > 0) {
                 page = t * kTile / p.block_size;
                 off = t * kTile - page * p.block_size;
-                item.first = at / quota;
-                item.nch = (at + nt - 1) / quota - item.first + 1;
-            } else {
-                next_pair();
             }
-            int blk = at + t < end ? table[page] : 0;
+            int blk = at + t < end ? table[page] : 0;  // loaded one tile ahead
 
             int stage = 0, qb = 0;
             uint32_t phase = 0;
@@ -459,7 +455,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
             bool ok = true;
             int first_flag = kFirst;
             while (at + t < end) {
-                const Header cur = item;
+                const int cur_b = b, cur_h = h, cur_at = at, cur_nt = nt;
                 const int tile = t, tile_ctx = ctx, tile_off = off, tile_blk = blk;
                 // Where the walk goes next.
                 off += kTile;
@@ -473,22 +469,28 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
                     break;
                 }
                 const bool in_cache = tile_blk >= 0 && tile_blk < p.num_blocks;
-                *reinterpret_cast<int4*>(&sm.tile[stage]) = make_int4(
-                    tile, first_flag | (last ? kLast : 0) | (in_cache ? 0 : kNoPage) | (qb ? kQBuf : 0), tile_ctx, 0);
-                if (last) *reinterpret_cast<int4*>(&sm.item[stage]) = make_int4(cur.b, cur.h, cur.first, cur.nch);
-                mbar_arrive_expect_tx(&sm.full[stage],
-                                      (in_cache ? uint32_t(kStageBytes) : 0u) + (first_flag ? q_bytes * p.lq : 0u));
+                mbar_expect_tx(&sm.full[stage],
+                               (in_cache ? uint32_t(kStageBytes) : 0u) + (first_flag ? q_bytes * p.lq : 0u));
                 if (in_cache) {
                     uint8_t* st = sm.stages[stage];
-                    const int64_t o = tile_blk * page_bytes + cur.h * head_bytes + tile_off * kRecord;
+                    const int64_t o = tile_blk * page_bytes + cur_h * head_bytes + tile_off * kRecord;
                     bulk_load_hint(st, p.k + o, kKvBytes, &sm.full[stage], pol);
                     bulk_load_hint(st + kKvBytes, p.v + o, kKvBytes, &sm.full[stage], pol);
                 }
                 if (first_flag) {
-                    const uint16_t* qsrc = p.q + int64_t(cur.b) * p.lq * p.q_stride + int64_t(cur.h) * p.group * kD;
+                    const uint16_t* qsrc = p.q + int64_t(cur_b) * p.lq * p.q_stride + int64_t(cur_h) * p.group * kD;
                     for (int j = 0; j < p.lq; ++j)
                         bulk_load(sm.qbuf[qb] + j * q_bytes, qsrc + int64_t(j) * p.q_stride, q_bytes, &sm.full[stage]);
                 }
+                // What the warps need with the tile is written while it is on its way.
+                *reinterpret_cast<int4*>(&sm.tile[stage]) = make_int4(
+                    tile, first_flag | (last ? kLast : 0) | (in_cache ? 0 : kNoPage) | (qb ? kQBuf : 0), tile_ctx, 0);
+                if (last) {
+                    const int first = cur_at / quota;
+                    *reinterpret_cast<int4*>(&sm.item[stage]) =
+                        make_int4(cur_b, cur_h, first, (cur_at + cur_nt - 1) / quota - first + 1);
+                }
+                mbar_arrive(&sm.full[stage]);
                 ++fills;
                 if (++stage == kStages) { stage = 0; phase ^= 1; }
                 first_flag = last ? kFirst : 0;
@@ -518,6 +520,15 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
     }
 
     // ---------------------------------------------------------------- consumers
+    // Rows without a cached token (CUDA-graph padding) have no tiles and get a zero output.
+    const int64_t row_vec = int64_t(p.lq) * p.hq * kD / 8;  // uint4 per batch row
+    for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
+        if (sm.lens[b] == 0) {
+            uint4* o = reinterpret_cast<uint4*>(p.out) + b * row_vec;
+            for (int64_t i = tid; i < row_vec; i += kConsumers) o[i] = make_uint4(0, 0, 0, 0);
+        }
+    }
+    if (begin >= end) return;
     const int g = lane >> 2, c = lane & 3;
     const int tok_warp = warp * kWarpTokens;
     // Byte offsets in a sub-tile's records: the rows this lane hands to ldmatrix (token lane & 7, group
@@ -940,7 +951,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
     }
 
     // The run's partial items (its first and its last), after the loop so that the merge's registers are
-    // not held beside it: publish this warp's share of each (one release fence per warp, cumulative over the
+    // not held beside it: publish this warp's share of each (one releasing count per warp, cumulative over the
     // warp barrier), then count it; the last chunk's warp of this number merges the share.  Groups are
     // counted and merged in what belongs to their second chunk's CTA, which has no other item.
     auto arrive_last = [&](int cta, int n) {
@@ -948,14 +959,12 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
         int last = 0;
         if (lane == 0) {
             int32_t* counter = &p.counters[cta * kWarps + warp];
-            __threadfence();
-            last = atomicAdd(counter, 1) == n - 1;
-            if (last) {
-                __threadfence();
-                *counter = 0;
-            }
+            last = atomic_inc_acq_rel(counter) == n - 1;
+            if (last) *counter = 0;
         }
-        return __shfl_sync(0xffffffffu, last, 0);
+        last = __shfl_sync(0xffffffffu, last, 0);
+        __syncwarp();
+        return last;
     };
 #pragma unroll 1
     for (int i = 0; i < 2; ++i) {
