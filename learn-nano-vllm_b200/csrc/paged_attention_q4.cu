@@ -45,7 +45,7 @@
 // bounded (kWaitLimitNs, or the test limit).
 //
 // What bounds it (512 sequences, 1.17 M tokens, 8 kv heads of 4 rows: 1.50 GB, 228 us at the measured
-// copy rate): 273 us, 158 M warp instructions, the vector pipes; held for a second it reaches the
+// copy rate): 272 us, 158 M warp instructions, the vector pipes; held for a second it reaches the
 // board's power cap, 1.74 GHz and 296 to 313 us.  A record costs its share of 270 instructions per
 // 16 tokens, 72 of them masks.  16 consumer warps per SM (104 registers each, taken from their
 // producers) issue more often, spill, and take 272 us; they would cost the short calls 2 us.
@@ -79,7 +79,7 @@ constexpr int kKvBytes = kTile * kRecord;  // keys (or values) of one stage
 constexpr int kStageBytes = 2 * kKvBytes;
 constexpr int kMaxBatch = 2048;
 // What a (sequence, kv head) pair costs beside its tiles, in tiles (decode of 512 sequences / verify of
-// 128: 273 / 131 us with 2, 275 / 138 with 1, 278 / 133 with 3, 282 / 134 with 4).
+// 128: 272 / 129 us with 2, 275 / 138 with 1, 277 / 130 with 3, 282 / 132 with 4).
 constexpr int kPairCost = 2;
 constexpr float kCodeUnit = 1.f / 16777216.f;  // 2^-24, the value of code 1 as an fp16 operand
 constexpr float kLazyMax = 8.f;  // log2 headroom before a row's running maximum is raised
