@@ -284,11 +284,11 @@ __device__ __forceinline__ float log_weight(float m, float den) {
     return den == 0.f ? -INFINITY : (den <= FLT_MAX ? m + fast_log2(den) : INFINITY);
 }
 
-// Up to 40 chunks of a split pair are merged at once; more in groups of group_of(nch) and what is left, whose
+// Up to 28 chunks of a split pair are merged at once; more in groups of group_of(nch) and what is left, whose
 // results, at most 16, are merged in turn.  (The whole call, at once / in groups: one sequence of 200k and
-// one kv head, 444 chunks, 43.5 / 20.6 us; 32k and two heads 21.9 / 14.7; 32k and eight, 52 chunks, 20.8 / 20.2; 8k and
-// eight, 33 chunks, 13.9 / 14.2.)
-__device__ __forceinline__ int group_of(int nch) { return nch <= 40 ? nch : max(8, (nch + 15) / 16); }
+// one kv head, 444 chunks, 43.1 / 19.3 us; 32k and two heads 20.9 / 13.6; 32k and eight, 52 chunks, 20.2 / 19.2; 4k and
+// eight, 32 chunks, 12.6 / 12.3; 3000 tokens, 24 chunks, 11.1 / 11.5.)
+__device__ __forceinline__ int group_of(int nch) { return nch <= 28 ? nch : max(8, (nch + 15) / 16); }
 
 // Partial results that are merged: number u lies in slot `head` (u = 0) or base + step * u.  The result goes to
 // the outputs of hd's pair (to < 0) or to slot `to`.
@@ -298,8 +298,8 @@ struct Merge {
 };
 
 // Merges this warp's share of each pass of kPassRows rows, kFlight chunks' loads in flight; called by the warp
-// that finished the last of them.  (3 chunks of a short sequence, the whole call: 9.3 us with 4 in flight, 10.3
-// with 16.)
+// that finished the last of them.  (3 chunks of a short sequence, the whole call: 8.5 us with 4 in flight, 9.3
+// with 16; 5 chunks 8.6 with 8, 9.1 with 16.)
 template <bool BF16, int NT, int kFlight>
 __device__ __forceinline__ void merge_share(const Params& p, const Header& hd, const Merge& mg, int warp, int lane) {
     using C = Cfg<NT>;
@@ -966,6 +966,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
         __syncwarp();
         return last;
     };
+    auto merge = [&](const Header& hd, const Merge& mg) {
+        if (mg.n <= 4) merge_share<BF16, NT, 4>(p, hd, mg, warp, lane);
+        else if (mg.n <= 8) merge_share<BF16, NT, 8>(p, hd, mg, warp, lane);
+        else merge_share<BF16, NT, 16>(p, hd, mg, warp, lane);
+    };
 #pragma unroll 1
     for (int i = 0; i < 2; ++i) {
         const Header hd = sm.part[warp][i];
@@ -977,13 +982,12 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
             const int n = grp == groups - 1 ? hd.nch - c0 : size;
             if (!arrive_last(cta, n)) continue;
             const int64_t at = 2 * int64_t(hd.first + c0);
-            merge_share<BF16, NT, 16>(p, hd, Merge{at + (grp == 0), at, 2 * int64_t(cta) + 1, 2, n}, warp, lane);
+            merge(hd, Merge{at + (grp == 0), at, 2 * int64_t(cta) + 1, 2, n});
             const int64_t to = 2 * int64_t(hd.first + 1) + 1;
             mg = Merge{to, to, -1, 2 * size, groups};
         }
         if (!arrive_last(hd.first, mg.n)) continue;
-        if (mg.n <= 4) merge_share<BF16, NT, 4>(p, hd, mg, warp, lane);
-        else merge_share<BF16, NT, 16>(p, hd, mg, warp, lane);
+        merge(hd, mg);
     }
 }
 
