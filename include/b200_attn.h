@@ -152,6 +152,13 @@ B200_API int32_t b200_gather_kvcache_q4(void* key, int64_t key_stride,
  */
 B200_API size_t b200_paged_attention_q4_workspace_size(int32_t query_len, int32_t group_size);
 
+/*
+ * Identifier of the CUDA-graph capture that `stream` takes part in (unique in
+ * the process), 0 if it is not being captured: calls captured on one stream
+ * can share a workspace that the graph zeroes once, as the Python wrapper's do.
+ */
+B200_API int32_t b200_stream_capture_id(void* stream, uint64_t* id);
+
 B200_API int32_t b200_paged_attention_q4(void* out, const void* q, int64_t q_stride_token,
                                 const void* k_cache, const void* v_cache,
                                 int32_t num_blocks, int32_t block_size,

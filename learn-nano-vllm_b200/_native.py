@@ -28,6 +28,7 @@ SIGNATURES = {
     "b200_gather_kvcache_q4": (_I32, [_P, _I64, _P, _I64, _P, _P, _P, _P, _I64, _I32, _I32, _I32, _I32, _I32, _I32,
                                       _I32, _I32, _P]),
     "b200_paged_attention_q4_workspace_size": (_SZ, [_I32, _I32]),
+    "b200_stream_capture_id": (_I32, [_P, _P]),
     "b200_paged_attention_q4": (_I32, [_P, _P, _I64, _P, _P, _I32, _I32, _P, _I64, _I32, _P, _I32, _I32, _I32, _I32,
                                        _I32, _F, _I32, _P, _SZ, _P]),
     "b200_workspace_error": (_I32, [_P, _P, ctypes.POINTER(ctypes.c_int32)]),

@@ -1015,6 +1015,17 @@ extern "C" size_t b200_paged_attention_q4_workspace_size(int32_t query_len, int3
     return rows > 16 ? 0 : workspace_bytes(int(rows));
 }
 
+extern "C" int32_t b200_stream_capture_id(void* stream, uint64_t* id) {
+    using namespace b200;
+    clear_error();
+    B200_REQUIRE(id, "stream_capture_id: null pointer");
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    unsigned long long capture = 0;
+    B200_CUDA_TRY(cudaStreamGetCaptureInfo(static_cast<cudaStream_t>(stream), &status, &capture));
+    *id = status == cudaStreamCaptureStatusActive ? capture : 0;
+    return B200_OK;
+}
+
 extern "C" int32_t b200_paged_attention_q4(void* out, const void* q, int64_t q_stride_token, const void* k_cache,
                                            const void* v_cache, int32_t num_blocks, int32_t block_size,
                                            const int32_t* block_tables, int64_t block_table_stride,

@@ -18,6 +18,7 @@ contracts (nanovllm/layers/attention.py:33-40, :64-74): they check their tensors
 current stream of the tensors' device and never synchronise the host (except
 `gather_kvcache_q4` without `total_tokens`).
 """
+import ctypes
 import threading
 
 import torch
@@ -198,6 +199,7 @@ def gather_kvcache_q4(k_cache: torch.Tensor, v_cache: torch.Tensor, cu_seqlens: 
 # ------------------------------------------------------------------ attention
 _ws_lock = threading.Lock()
 _workspaces: dict[tuple, torch.Tensor] = {}
+_captures: dict[tuple, tuple] = {}
 
 
 def q4_workspace_size(query_len: int, group: int) -> int:
@@ -210,19 +212,27 @@ def q4_workspace(device: torch.device, query_len: int, group: int) -> torch.Tens
     """The split-K workspace of a call on the current stream, its control words and counters zero.
 
     Eager calls keep one per (device, stream), for up to 16 query rows: calls of one stream run one
-    after another and leave it re-armed.  A call that is being captured gets its own from the graph's
-    memory pool, zeroed by the graph itself, so that graphs replayed at the same time share nothing."""
+    after another and leave it re-armed.  The calls captured on one stream into one graph share one from
+    the graph's memory pool, zeroed once by the graph itself, so that graphs replayed at the same time share
+    nothing."""
     index = device.index if device.index is not None else torch.cuda.current_device()
     with torch.cuda.device(index):
-        return _workspace(index, query_len * group)
+        assert q4_workspace_size(query_len, group) > 0, f"{query_len} queries of {group} heads: 1 to 16 rows per kv head"
+        return _workspace(index)
 
 
-def _workspace(index, rows):
-    if torch.cuda.is_current_stream_capturing():
-        ws = torch.empty(q4_workspace_size(rows, 1), dtype=torch.uint8, device=torch.device("cuda", index))
-        ws[:_CONTROL_BYTES].zero_()
-        return ws
+def _workspace(index):
     key = (index, _raw_stream(index))
+    if torch.cuda.is_current_stream_capturing():
+        capture = ctypes.c_uint64()
+        check(lib().b200_stream_capture_id(key[1], ctypes.addressof(capture)), "stream_capture_id")
+        held = _captures.get(key)
+        if held is None or held[0] != capture.value:
+            # Held until the stream's next capture: the graph's pool must not hand it out again meanwhile.
+            ws = torch.empty(q4_workspace_size(16, 1), dtype=torch.uint8, device=torch.device("cuda", index))
+            ws[:_CONTROL_BYTES].zero_()
+            held = _captures[key] = capture.value, ws
+        return held[1]
     ws = _workspaces.get(key)
     if ws is None:
         with _ws_lock:
@@ -279,12 +289,11 @@ def flash_attn_with_kvcache_q4(q, k_cache, v_cache, cache_seqlens=None, block_ta
         _explain_attention(q, k_cache, v_cache, cache_seqlens, block_table, causal, out)
     Hkv = cs[1]
     if workspace is None:
-        rows = min(Lq * (Hq // Hkv), 16)
         if _current_device() == dev:
-            workspace = _workspace(dev, rows)
+            workspace = _workspace(dev)
         else:
             with torch.cuda.device(dev):
-                workspace = _workspace(dev, rows)
+                workspace = _workspace(dev)
     else:
         assert workspace.dtype is _U8 and workspace.get_device() == dev and workspace.is_contiguous(), \
             "the workspace must be contiguous uint8 on q's device"

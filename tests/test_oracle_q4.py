@@ -167,6 +167,7 @@ def test_c_abi_refusals(pkg):
     for kw, rc in [(dict(n=0), 0), (dict(s=0), 0), (dict(n=-1), ARG), (dict(s=-1), ARG), (dict(cu=None), ARG),
                    (dict(btw=0), ARG), (dict(bts=-1), ARG), (dict(d=96), UNS), (dict(dt=7), UNS)]:
         assert lib.b200_gather_kvcache_q4(*{**ga, **kw}.values()) == rc, kw
+    assert lib.b200_stream_capture_id(None, None) == ARG
     pa = dict(out=a, q=a, qs=512, kc=a, vc=a, nb=1, bs=128, bt=a, bts=1, btw=1, cl=a, b=1, lq=1, hq=4, hkv=2, d=128,
               sc=0.1, dt=1, ws=a, wb=1 << 24, st=None)
     for kw, rc in [(dict(b=0), 0), (dict(b=-1), ARG), (dict(q=None), ARG), (dict(hq=3), ARG), (dict(hkv=0), ARG),

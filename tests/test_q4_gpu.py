@@ -525,6 +525,49 @@ def test_two_graphs_replayed_at_once(pkg):
     del graphs
 
 
+def test_calls_of_one_graph_share_a_workspace(pkg):
+    """Decode and verify calls of one capture take turns on one workspace; another capture, another stream of
+    the same capture and the eager calls have their own."""
+    a, b = make([9000, 300], 8, 2, seed=24), make([8000, 700], 8, 2, lq=3, seed=25)
+    f = lambda x, out: pkg.flash_attn_with_kvcache_q4(x[0], x[1], x[2], cache_seqlens=x[3], block_table=x[4], out=out)
+    want = [f(x, None) for x in (a, b)]
+    s, side = torch.cuda.Stream(), torch.cuda.Stream()
+    held, graphs, results = [], [], []
+    for _ in range(2):
+        outs = [torch.zeros_like(w) for w in want * 2]
+        forked = torch.zeros_like(want[0])
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            ws = pkg.q4_workspace(torch.device("cuda"), 1, 4)
+            side.wait_stream(s)
+            with torch.cuda.stream(side):
+                f(a, forked)
+                other = pkg.q4_workspace(torch.device("cuda"), 1, 4)
+            for x, o in zip((a, b) * 2, outs):
+                f(x, o)
+            assert pkg.q4_workspace(torch.device("cuda"), 3, 4).data_ptr() == ws.data_ptr()
+            s.wait_stream(side)
+        held += [ws, other]
+        graphs.append(g)
+        results.append(outs + [forked])
+    with torch.cuda.stream(s):
+        held.append(pkg.q4_workspace(torch.device("cuda"), 1, 4))
+    assert len({w.data_ptr() for w in held}) == 5
+    for _ in range(3):
+        for outs in results:
+            for o in outs:
+                o.fill_(7)
+        torch.cuda.synchronize()
+        for g, st in zip(graphs, (s, side)):
+            with torch.cuda.stream(st):
+                g.replay()
+        torch.cuda.synchronize()
+        for outs in results:
+            assert all(torch.equal(o, w) for o, w in zip(outs, want * 2 + want[:1]))
+    del graphs
+
+
 def test_captured_decode_step(pkg):
     """store + attention of a padded batch, captured once and replayed with new tokens, lengths and tables."""
     B, hq, hkv, bs, nb = 8, 16, 8, 128, 40
