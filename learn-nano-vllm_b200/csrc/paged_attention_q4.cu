@@ -45,7 +45,7 @@
 // bounded (kWaitLimitNs, or the test limit).
 //
 // What bounds it (512 sequences, 1.17 M tokens, 8 kv heads of 4 rows: 1.50 GB, 228 us at the measured
-// copy rate): 272 us, 158 M warp instructions, the vector pipes; held for a second it reaches the
+// copy rate): 267 us, 157 M warp instructions, the vector pipes; held for a second it reaches the
 // board's power cap, 1.74 GHz and 296 to 313 us.  A record costs its share of 270 instructions per
 // 16 tokens, 72 of them masks.  16 consumer warps per SM (104 registers each, taken from their
 // producers) issue more often, spill, and take 272 us; they would cost the short calls 2 us.
@@ -83,6 +83,7 @@ constexpr int kMaxBatch = 2048;
 constexpr int kPairCost = 2;
 constexpr float kCodeUnit = 1.f / 16777216.f;  // 2^-24, the value of code 1 as an fp16 operand
 constexpr float kLazyMax = 8.f;  // log2 headroom before a row's running maximum is raised
+constexpr float kReach = 2048.f;  // what value parameters times 2^-E may reach before E is raised
 constexpr float kNone = -1e30f;  // reference of a row that has met no token
 constexpr int kExpMax = 60;      // bound of |E| and of the query rows' exponents
 
@@ -547,15 +548,14 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
     __syncwarp();
     int stage = 0;
     uint32_t phase = 0, cphase = 0;
-    // Query rows 8 nt + 2 c + e: reference (log2), factor of the scores, limit.
+    // Query rows 8 nt + 2 c + e: reference (log2), factor of the scores.  (What the loop can recompute is not held:
+    // a limit per row and the reach that E allows cost 4 us of 271, and 2 of the verify call.)
     float r_ref[NT][2], f_row[NT][2];
-    int lim[NT][2];
-    int lim_min = 0;
     uint32_t qf[kGroups][NT][4], qs[NT][2];  // B operands of row 8 nt + g: q (two steps of a group), (0, sum q) of group c
     // O^T fragments (16 dims x 8 rows in units of 2^-24), and the product with the parameter words:
     // its row g is sum_t p * (half-word g), rows 8.. are sum_t p.
     float o[kGroups][2][NT][4], om[NT][4];
-    float unit = 1.f, reach_lim = 0.f;  // 2^-E, and the reach of value parameters that E allows
+    float unit = 1.f;  // 2^-E
     bool reading = false;            // the last combine's shared memory may still be read by other warps
     while (true) {
         // Exit decisions are warp-uniform (the lanes' waits can disagree at the limit).
@@ -615,10 +615,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
                 const float fm = fmaxf(p.scale_log2 * exp2_int(eq) * (kMinFirst ? 1.f / kCodeUnit : 1.f), 1e-30f);
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const int rw = 8 * nt + 2 * c + e;
                     f_row[nt][e] = __shfl_sync(0xffffffffu, fm, (2 * c + e) * 4);  // a lane of row rw
-                    // Padding rows see the whole context: only rows that exist mask.
-                    lim[nt][e] = rw < p.rows ? ctx - p.lq + ((rw * p.group_inv) >> 16) : ctx - 1;
                     r_ref[nt][e] = kNone;
                 }
 #pragma unroll
@@ -630,10 +627,13 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
 #pragma unroll
                         for (int e = 0; e < 4; ++e) o[j][t][nt][e] = 0.f;
             }
-            lim_min = ctx - p.lq;  // the smallest: row 0's
             unit = exp2_int(kExpMax);
-            reach_lim = 0.f;
         }
+        // Last token that row 8 nt + 2 c + e sees.  Padding rows see the whole context: only rows that exist mask.
+        auto lim = [&](int nt, int e) {
+            const int rw = 8 * nt + 2 * c + e;
+            return rw < p.rows ? ctx - p.lq + ((rw * p.group_inv) >> 16) : ctx - 1;
+        };
         bool wrote = false;
         {
             // Records past the context may hold anything (a NaN scale times a probability of 0 is
@@ -714,7 +714,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
-                            if (tok_base + 16 * u + g + (e >> 1) * 8 > lim[nt][e & 1]) x[u][nt][e] = -INFINITY;
+                            if (tok_base + 16 * u + g + (e >> 1) * 8 > lim(nt, e & 1)) x[u][nt][e] = -INFINITY;
             }
             float y_max = -INFINITY;
 #pragma unroll
@@ -725,18 +725,17 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
                                               f_row[nt][e], -r_ref[nt][e]));
             const uint4 look = *reinterpret_cast<const uint4*>(vb + look_off);  // value parameters of token `lane`
             const float reach = reach_of<BF16>(look);
-            if (__any_sync(0xffffffffu, y_max > kLazyMax || reach > reach_lim)) {
+            if (__any_sync(0xffffffffu, y_max > kLazyMax || reach * unit > kReach)) {
                 // Rare: raise E to the value parameters of this tile, the rows' maxima to its scores.
                 float top = reach;
 #pragma unroll
                 for (int sh = 1; sh <= 16; sh <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, sh));
                 float drop = 1.f;  // 2^-(rise of E)
-                if (top > reach_lim) {
+                if (top * unit > kReach) {
                     const int old = 127 - (__float_as_int(unit) >> 23);  // E
                     const int en = min(max((__float_as_int(top) >> 23) - 127 - 6, old), kExpMax);
                     drop = exp2_int(old - en);
                     unit = exp2_int(-en);
-                    reach_lim = en == kExpMax ? INFINITY : exp2_int(en + 11);
                 }
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
@@ -774,7 +773,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
                         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                             for (int e = 0; e < 2; ++e)
-                                if (g == 2 * j + 1 && t <= lim[nt][e]) om[nt][e] = __int_as_float(0x7fffffff);
+                                if (g == 2 * j + 1 && t <= lim(nt, e)) om[nt][e] = __int_as_float(0x7fffffff);
                     }
                 }
             }
@@ -846,7 +845,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
                 }
             }
             };
-            if (__any_sync(0xffffffffu, tok_base + 31 > lim_min)) step(std::true_type{});
+            if (__any_sync(0xffffffffu, tok_base + 31 > ctx - p.lq)) step(std::true_type{});
             else step(std::false_type{});
         }
         if (wrote) fence_proxy_async_smem();
