@@ -46,7 +46,7 @@
 //
 // What bounds it (512 sequences, 1.17 M tokens, 8 kv heads of 4 rows: 1.50 GB, 228 us at the measured
 // copy rate): 267 us, 157 M warp instructions, the vector pipes; held for a second it reaches the
-// board's power cap, 1.74 GHz and 296 to 313 us.  A record costs its share of 270 instructions per
+// board's power cap, 1.74 GHz and 290 to 313 us.  A record costs its share of 268 instructions per
 // 16 tokens, 72 of them masks.  16 consumer warps per SM (104 registers each, taken from their
 // producers) issue more often, spill, and take 272 us; they would cost the short calls 2 us.
 #include <atomic>
