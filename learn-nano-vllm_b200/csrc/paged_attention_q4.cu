@@ -48,7 +48,7 @@
 // copy rate): 267 us, 157 M warp instructions, the vector pipes; held for a second it reaches the
 // board's power cap, 1.74 GHz and 290 to 313 us.  A record costs its share of 268 instructions per
 // 16 tokens, 72 of them masks.  16 consumer warps per SM (104 registers each, taken from their
-// producers) issue more often, spill, and take 272 us; they would cost the short calls 2 us.
+// producers) issue more often, spill, and gain nothing; they would cost the short calls 2 us.
 #include <atomic>
 #include <cfloat>
 #include <climits>
