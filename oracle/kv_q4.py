@@ -147,3 +147,70 @@ def tolerance(want, bound, bf16):
         2^-11 of at most 15 s, and below 2^-14 half of 2^-24 in units of at most R / 64: m 2^-27 R;
       * 2^-20 R for the fp32 sums and exponentials."""
     return np.abs(want) * (2.0 ** -8 if bf16 else 2.0 ** -11) + bound + (2.0 ** -130 if bf16 else 2.0 ** -25)
+
+
+def attention_bound(q, k_rec, v_rec, block_tables, context_lens, scale, bf16):
+    """As attention(), with a bound that is each element's own: its group's parameters under the
+    row's own probabilities, in place of the largest value that the row may meet.
+
+    With w_t a row's probabilities, o its output, and s_t, m_t, n_t the scale and minimum of the element's
+    group and its code at token t (v_t = n_t s_t + m_t), N tokens seen, R the group's largest max(16 s, |m|):
+      * scores off by d_t move a weighted mean by sum w_t d_t (v_t - o).  Products of 16-bit
+        operands are exact, sums fp32, and sum(q) is held to 2^-23 of sum |q|: d_t is 2^-20 of
+        scale * sum |q| (n s + |m|).  Queries are 16-bit operands in units of a power of two in which the
+        row's largest is at least 1/2: below 2^-14 half a step is 2^-25, so each element adds 2^-24 max|q| n s;
+      * a matrix product of 16 terms cuts each term (and the running sum) at 2^-25 of the largest exponent
+        sum among its operands, in which a code that is a subnormal counts as 2^-14: 16 cuts of 2^-25 2^-14 are
+        2^-11 of what code 1, 2^-24, makes of the largest other operand.  Scores: 2^-11 s max|q| for each of a
+        group's two products.  Values: 2^-11 of the largest p s among each 16 tokens;
+      * exponentials: 2^-18 of p (ex2.approx, and a fused exponent rounded at a magnitude below 64);
+      * p to fp16, the same in numerator and sum: 2^-11 of p (fp16 models carry the rest: 2^-21), and
+        half of 2^-24 below 2^-14 where the row's largest p is at least 2^8: 2^-33 of the sum per token;
+      * p s to fp16: 2^-11 of p s n (2^-21); below 2^-14 half of 2^-24 times a code of 15, in units
+        of at most R / 8, of a sum that is at least 2^8: 2^-32 R per token;
+      * s and m in fp16 units of at most R / 8: exact but for 2^-25 of a unit: (15 + 1) 2^-28 R < 2^-23 R;
+      * fp32 sums, truncated at each step by at most 2^-23 of the sum of their terms' magnitudes (n s + |m|):
+        a warp meets a quarter of the tokens, 16 (fp16 models: 8) at a time, and up to eight more steps
+        join the parts."""
+    B, lq, hq, d = q.shape
+    nb, hkv, bs, _ = k_rec.shape
+    g = hq // hkv
+    out, bound = np.zeros(q.shape), np.zeros(q.shape)
+    rel = 2.0 ** -11 if bf16 else 2.0 ** -21
+    for b in range(B):
+        n = min(int(context_lens[b]), block_tables.shape[1] * bs)
+        if n <= 0:
+            continue
+        pages = np.asarray(block_tables[b, :(n + bs - 1) // bs])
+        inside = (pages >= 0) & (pages < nb)
+        safe = np.where(inside, pages, 0)
+        for h in range(hkv):
+            kr, vr = (np.where(inside[:, None, None], c[safe, h], 0).astype(np.uint8).reshape(-1, RECORD)[:n]
+                      for c in (k_rec, v_rec))
+            (nk, sk, mk), (nv, sv, mv) = unpack(kr, bf16), unpack(vr, bf16)
+            ks, vs = (nk * sk[..., None]).reshape(n, d), (nv * sv[..., None]).reshape(n, d)  # n s
+            K, V = values(kr, bf16), values(vr, bf16)
+            km, vm = np.repeat(np.abs(mk), GROUP, 1), np.repeat(np.abs(mv), GROUP, 1)
+            for i in range(lq):
+                m = n - lq + i + 1
+                if m <= 0:
+                    continue
+                qi = q[b, i, h * g:(h + 1) * g]                                   # [g, d]
+                s = (qi @ K[:m].T) * scale
+                w = np.exp(s - s.max(-1, keepdims=True))
+                w /= w.sum(-1, keepdims=True)
+                o = w @ V[:m]
+                dt = scale * (2.0 ** -20 * (np.abs(qi) @ (ks[:m] + km[:m]).T)
+                              + 2.0 ** -24 * np.abs(qi).max(-1, keepdims=True) * ks[:m].sum(-1)
+                              + 2.0 ** -10 * np.abs(qi).reshape(g, 4, GROUP).max(-1) @ sk[:m].T)
+                we = w * (1.1 * dt + rel + 2.0 ** -18)
+                R = np.repeat(np.maximum(16 * sv[:n], np.abs(mv[:n])).max(0), GROUP)
+                steps = 8 + m / (64 if bf16 else 32)
+                e = we @ np.abs(V[:m]) + we.sum(-1, keepdims=True) * np.abs(o)
+                e += 2.0 ** -33 * (np.abs(V[:m]).sum(0) + m * np.abs(o))
+                e += rel * (w @ vs[:m]) + (m * 2.0 ** -32 + 2.0 ** -23) * R
+                e += steps * 2.0 ** -23 * (w @ (vs[:m] + vm[:m]))
+                ps = np.pad(w[:, :, None] * sv[:m], ((0, 0), (0, -m % 16), (0, 0))).reshape(g, -1, 16, 4)
+                e += 2.0 ** -11 * np.repeat(ps.max(2).sum(1), GROUP, -1)
+                out[b, i, h * g:(h + 1) * g], bound[b, i, h * g:(h + 1) * g] = o, e
+    return out, bound

@@ -1,0 +1,51 @@
+"""Attention over 4-bit caches against each element's own error bound."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import kv_q4
+from tests.test_q4_gpu import BF16, F16, make, oracle_records
+
+pytestmark = pytest.mark.gpu
+
+
+def close(pkg, q, kc, vc, cl, bt, scale=128 ** -0.5, what="", rows=slice(None)):
+    """The call within its bound at the batch rows `rows`."""
+    out = pkg.flash_attn_with_kvcache_q4(q, kc, vc, cache_seqlens=cl, block_table=bt, softmax_scale=scale)
+    bf = q.dtype == BF16
+    rows = torch.arange(len(q), device="cuda")[rows] if isinstance(rows, slice) else torch.tensor(rows, device="cuda")
+    q, cl, bt, out = q[rows], cl[rows], bt[rows], out[rows]
+    want, bound = kv_q4.attention_bound(q.double().cpu().numpy(), kc.cpu().numpy(), vc.cpu().numpy(), bt.cpu().numpy(),
+                                        cl.cpu().numpy(), scale, bf)
+    err, tol = np.abs(out.double().cpu().numpy() - want), kv_q4.tolerance(want, bound, bf)
+    worst = np.unravel_index(np.nan_to_num(err / tol, nan=np.inf).argmax(), err.shape)
+    assert (err <= tol).all(), f"{what}: at {worst} {err[worst] / tol[worst]:.2f} of the bound, want {want[worst]}"
+
+
+def cache_of(x):
+    """A cache [nb, h, bs, 80] of rows [nb, h, bs, 128]."""
+    return torch.from_numpy(oracle_records(x.reshape(x.shape[0], -1, 128)).reshape(*x.shape[:3], 80)).cuda()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("lq,hq,hkv", [(1, 16, 8), (1, 8, 1), (5, 16, 8), (1, 1, 1)])
+def test_ordinary_rows(pkg, dtype, lq, hq, hkv):
+    close(pkg, *make([700, 65, 3001, 5], hq, hkv, lq=lq, dtype=dtype, seed=hq + lq), what="ordinary")
+    close(pkg, *make([20000, 129], hq, hkv, lq=lq, dtype=dtype, kscale=3.0, vscale=50.0, seed=hq + lq), what="peaked, split")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_small_tokens_beside_large_ones(pkg, dtype):
+    """Pages whose values differ by 2^12, heads that attend to one page each."""
+    nb, bs, lows = 4, 128, (0, -12, -6, -9)
+    g = torch.Generator(device="cuda").manual_seed(52)
+    rows = lambda s: torch.randn(nb, 1, bs, 128, generator=g, device="cuda") * s
+    k, v = rows(0.3), rows(1.0) + 0.1
+    q = torch.zeros(1, 1, 4, 128, device="cuda")
+    for p, e in enumerate(lows):
+        k[p, ..., 32 * p:32 * p + 32] += 4.0
+        q[0, 0, p, 32 * p:32 * p + 32] = 1.0
+        v[p] *= 2.0 ** e
+    bt = torch.arange(nb, dtype=torch.int32, device="cuda")[None]
+    cl = torch.tensor([nb * bs - 3], dtype=torch.int32, device="cuda")
+    close(pkg, q.to(dtype), cache_of(k.to(dtype)), cache_of(v.to(dtype)), cl, bt, scale=0.25, what="pages apart")
