@@ -24,9 +24,9 @@
 // would show both, carry the rest of p and of p s in a second product (0.00023 from 64 bits
 // relative, 0.00034 without; the output's own rounding is 0.0002).  Sums and maxima are fp32.
 //
-// Ranges.  p = 2^(x - r) with r the lazily raised running maximum, so p <= 2^kLazyMax.  The value
-// parameters enter as 2^-E of themselves, where E follows the largest max(16 s, |m|) the warp has
-// met (16 s 2^-E below 2^7 when E is set, raised beyond 2^11).  Queries are scaled by a power of
+// Ranges.  p = 2^(x - r) with r lazily raised to 2^8 below the running maximum, so p <= 2^kLazyMax.  The
+// value parameters enter as 2^-E of themselves, where E follows the largest max(16 s, |m|) the warp
+// has met (below 2^4 in these units when E is set, raised beyond 2^7).  Queries are scaled by a power of
 // two per row (largest element in [8, 16)), exactly but for elements below 2^-18 of it.
 //
 // Work split.  The tiles of 128 tokens of all (sequence, kv head) pairs in a row, sequence by
@@ -82,8 +82,14 @@ constexpr int kMaxBatch = 2048;
 // 128: 272 / 129 us with 2, 275 / 138 with 1, 277 / 130 with 3, 282 / 132 with 4).
 constexpr int kPairCost = 2;
 constexpr float kCodeUnit = 1.f / 16777216.f;  // 2^-24, the value of code 1 as an fp16 operand
-constexpr float kLazyMax = 8.f;  // log2 headroom before a row's running maximum is raised
-constexpr float kReach = 2048.f;  // what value parameters times 2^-E may reach before E is raised
+// A row's reference is set kTop (log2) below its maximum and raised once a score exceeds it by kLazyMax: the
+// largest p lies in [2^8, 2^12].  fp16 ends at 2^-25, so a token keeps a weight down to 2^-33 of the largest one's:
+// a long tail behind one token of a far larger score is not lost.  (p s stays below 2^15: kReach.)
+constexpr float kTop = 8.f;
+constexpr float kLazyMax = 12.f;
+// What value parameters (16 s, |m|) times 2^-E may reach before E is raised, to where they lie in [2^kUnitBits, 2 * that).
+constexpr float kReach = 128.f;
+constexpr int kUnitBits = 3;
 constexpr float kNone = -1e30f;  // reference of a row that has met no token
 constexpr int kExpMax = 60;      // bound of |E| and of the query rows' exponents
 
@@ -733,7 +739,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
                 float drop = 1.f;  // 2^-(rise of E)
                 if (top * unit > kReach) {
                     const int old = 127 - (__float_as_int(unit) >> 23);  // E
-                    const int en = min(max((__float_as_int(top) >> 23) - 127 - 6, old), kExpMax);
+                    const int en = min(max((__float_as_int(top) >> 23) - 127 - kUnitBits, old), kExpMax);
                     drop = exp2_int(old - en);
                     unit = exp2_int(-en);
                 }
@@ -745,7 +751,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
 #pragma unroll
                         for (int sh = 4; sh <= 16; sh <<= 1) tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, sh));
                         tm *= f_row[nt][e];
-                        const float ro = r_ref[nt][e], rn = fmaxf(ro, tm == -INFINITY ? kNone : tm);
+                        const float ro = r_ref[nt][e], rn = fmaxf(ro, tm == -INFINITY ? kNone : tm - kTop);
                         const float alpha = ro == kNone ? 0.f : fast_exp2(ro - rn), alpha_v = alpha * drop;
                         r_ref[nt][e] = rn;
                         om[nt][e] *= alpha_v;

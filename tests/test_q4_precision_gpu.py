@@ -49,3 +49,26 @@ def test_small_tokens_beside_large_ones(pkg, dtype):
     bt = torch.arange(nb, dtype=torch.int32, device="cuda")[None]
     cl = torch.tensor([nb * bs - 3], dtype=torch.int32, device="cuda")
     close(pkg, q.to(dtype), cache_of(k.to(dtype)), cache_of(v.to(dtype)), cl, bt, scale=0.25, what="pages apart")
+
+
+@pytest.mark.parametrize("dtype,n,lq,nats", [(BF16, 4000, 1, 17.5), (BF16, 4000, 1, 16.0), (BF16, 2000, 4, 17.0), (F16, 4000, 1, 17.0),
+                                             (F16, 3000, 3, 16.0)])
+def test_tail_behind_one_token(pkg, dtype, n, lq, nats):
+    """A first token far above all others in score and with values of zero: what is left of the output is the
+    tail, thousands of tokens with probabilities around 2^-24.  Enough sequences (of the same pages) that
+    none is split, so that the warp that meets the first token meets a quarter of its sequence's tail."""
+    bs, hkv, g, B = 256, 8, 4, 80
+    nb = -(-n // bs)
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    scale = 128 ** -0.5
+    base = torch.randn(hkv, 1, 1, 128, generator=gen, device="cuda")
+    q = base.view(hkv, 1, 128) + 0.05 * torch.randn(B, lq, hkv, g, 128, generator=gen, device="cuda")
+    k = 0.05 * torch.randn(nb, hkv, bs, 128, generator=gen, device="cuda")
+    v = torch.randn(nb, hkv, bs, 128, generator=gen, device="cuda") * 0.3 + 1
+    k[0, :, 0] = (base * (nats / scale) / (base * base).sum(-1, keepdim=True))[:, 0, 0]
+    v[0, :, 0] = 0
+    q = q.to(dtype).view(B, lq, hkv * g, 128)
+    kc, vc = cache_of(k.to(dtype)), cache_of(v.to(dtype))
+    bt = torch.arange(nb, dtype=torch.int32, device="cuda").expand(B, nb)
+    cl = torch.full((B,), n, dtype=torch.int32, device="cuda")
+    close(pkg, q, kc, vc, cl, bt, what=f"tail of {n}", rows=(0, 1, 37, B - 1))
