@@ -148,7 +148,9 @@ B200_API int32_t b200_gather_kvcache_q4(void* key, int64_t key_stride,
  * statistics and sums are fp32; the probabilities p (and p * s, for the product
  * with the codes) are rounded to fp16, and fp16 models add the products of what
  * the rounding left.  Tokens count down to 2^-33 of the weight of the token with
- * the largest score.  Queries, stored scales and stored minima are expected
+ * the largest score.  Value parameters (16 s and m) are held to 2^-28 of the
+ * largest among the sequence's, within each group of dimensions on its own.
+ * Queries, stored scales and stored minima are expected
  * between 2^-60 and 2^60 in magnitude, or zero.
  */
 B200_API size_t b200_paged_attention_q4_workspace_size(int32_t query_len, int32_t group_size);

@@ -7,7 +7,9 @@
 // The codes themselves are the matrix operands: a nibble in the low bits of an fp16 lane is the
 // subnormal n * 2^-24 (16 n * 2^-24 one nibble up), exactly, so that a mask turns a word of
 // codes into operands of mma.sync.m16n8k16 and nothing is converted.  The powers of two are
-// undone in fp32; the queries that meet a second nibble carry a factor 1/16.
+// undone in fp32; the queries that meet a second nibble carry a factor 1/16.  (A product of 16 terms cuts
+// each at 2^-25 of the largest exponent sum of its operands, in which a subnormal counts as 2^-14: what is
+// lost is below 2^-15 of code 1 times the largest other operand, per term.)
 //   * Tokens are the M of both products' operands: S^T = K Q^T and O^T = V^T (P s)^T, query rows
 //     their N of 8.  ldmatrix hands lane (g, c) word c of token g's four groups, the transposed form
 //     half-word g of tokens 2 c and 2 c + 1: one nibble per dimension (token) in either half of a
@@ -25,9 +27,10 @@
 // relative, 0.00034 without; the output's own rounding is 0.0002).  Sums and maxima are fp32.
 //
 // Ranges.  p = 2^(x - r) with r lazily raised to 2^8 below the running maximum, so p <= 2^kLazyMax.  The
-// value parameters enter as 2^-E of themselves, where E follows the largest max(16 s, |m|) the warp
-// has met (below 2^4 in these units when E is set, raised beyond 2^7).  Queries are scaled by a power of
-// two per row (largest element in [8, 16)), exactly but for elements below 2^-18 of it.
+// value parameters enter as 2^-E of themselves, one E per group, which follows the group's largest
+// max(16 s, |m|) that the warp has met (below 2^4 in these units when E is set, raised beyond 2^7): a
+// group keeps its precision beside far larger ones.  Queries are scaled by a power of two per row
+// (largest element in [8, 16)), exactly but for elements below 2^-18 of it.
 //
 // Work split.  The tiles of 128 tokens of all (sequence, kv head) pairs in a row, sequence by
 // sequence, are cut into equal runs (a pair counts kPairCost tiles more for its combine), one per
@@ -155,7 +158,6 @@ struct Smem {
     float co[kWarps][Cfg<NT>::kPassRows][kRowPad];
     float cm[kWarps][Cfg<NT>::kPassRows];
     float cl[kWarps][Cfg<NT>::kPassRows];
-    alignas(16) uint32_t ones[4];  // a row of fp16 ones
     TileHeader tile[kStages];
     Header item[kStages];          // with an item's last tile
     Header part[kWarps][2];        // the run's partial items, as each warp left them
@@ -244,17 +246,18 @@ __device__ __forceinline__ uint32_t fma_f16x2(uint32_t a, uint32_t b, uint32_t c
     return d;
 }
 
-// max(16 s, |m|) over four parameter words (NaNs apart).
+// The larger magnitudes of two pairs (their signs are no matter); a NaN beside a number is dropped.
 template <bool BF16>
-__device__ __forceinline__ float reach_of(const uint4& w) {
-    auto maxabs = [](uint32_t a, uint32_t b) {  // the larger magnitudes; their signs are no matter
-        uint32_t d;
-        if constexpr (BF16) asm("max.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-        else asm("max.xorsign.abs.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-        return d;
-    };
-    const uint32_t m = maxabs(maxabs(w.x, w.y), maxabs(w.z, w.w));
-    return fmaxf(fabsf(lo_f<BF16>(m)) * 16.f, fabsf(hi_f<BF16>(m)));
+__device__ __forceinline__ uint32_t max_abs(uint32_t a, uint32_t b) {
+    uint32_t d;
+    if constexpr (BF16) asm("max.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    else asm("max.xorsign.abs.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+
+// Two transposed 8x8 matrices of 16-bit elements; lanes 0-15 hand their rows.
+__device__ __forceinline__ void ldsm_x2_t(uint32_t& a, uint32_t& b, uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0,%1}, [%2];" : "=r"(a), "=r"(b) : "r"(addr));
 }
 
 // Barrier of the consumer threads, bounded.  False, for the whole warp alike, when a lane's wait ran out.
@@ -375,7 +378,6 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
         }
         mbar_init(&sm.cbar, kConsumers);
         sm.err = 0;
-        for (int i = 0; i < 4; ++i) sm.ones[i] = 0x3c003c00u;
         fence_mbar_init();
     }
 
@@ -539,13 +541,12 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
     const int g = lane >> 2, c = lane & 3;
     const int tok_warp = warp * kWarpTokens;
     // Byte offsets in a sub-tile's records: the rows this lane hands to ldmatrix (token lane & 7, group
-    // lane >> 3; the parameters of token lane & 15; transposed, those of token (lane & 7) + 8 (lane >> 4)
-    // or a row of ones), the parameters of token g, and those this lane looks over.
+    // lane >> 3; the parameters of token lane & 15; transposed, those of token `lane` of both sub-tiles),
+    // and the parameters of token g.
     const uint32_t frag_off = uint32_t(lane & 7) * kRecord + (lane >> 3) * 16;
     const uint32_t par_off = uint32_t(g) * kRecord + q4::kParams;
     const uint32_t word_off = uint32_t(lane & 15) * kRecord + q4::kParams;
-    const uint32_t trans_off = uint32_t((lane & 7) + (lane >> 4) * 8) * kRecord + q4::kParams;
-    const uint32_t look_off = uint32_t(lane) * kRecord + q4::kParams;
+    const uint32_t trans_off = uint32_t(lane) * kRecord + q4::kParams;
     // Scores in units of 2^-24, which the minima start as the MMAs' result; fp16 sums of q do not go down to
     // that unit, and 16 rows would spill (131.5 us against 133.4 for the verify call): there they join last.
     constexpr bool kMinFirst = BF16 && NT == 1;
@@ -561,7 +562,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
     // O^T fragments (16 dims x 8 rows in units of 2^-24), and the product with the parameter words:
     // its row g is sum_t p * (half-word g), rows 8.. are sum_t p.
     float o[kGroups][2][NT][4], om[NT][4];
-    float unit = 1.f;  // 2^-E
+    float unit = 1.f;  // 2^-E of group g >> 1
     bool reading = false;            // the last combine's shared memory may still be read by other warps
     while (true) {
         // Exit decisions are warp-uniform (the lanes' waits can disagree at the limit).
@@ -729,13 +730,16 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
                 for (int e = 0; e < 2; ++e)
                     y_max = fmaxf(y_max, fmaf(max3f(fmaxf(x[0][nt][e], x[0][nt][2 + e]), x[1][nt][e], x[1][nt][2 + e]),
                                               f_row[nt][e], -r_ref[nt][e]));
-            const uint4 look = *reinterpret_cast<const uint4*>(vb + look_off);  // value parameters of token `lane`
-            const float reach = reach_of<BF16>(look);
-            if (__any_sync(0xffffffffu, y_max > kLazyMax || reach * unit > kReach)) {
-                // Rare: raise E to the value parameters of this tile, the rows' maxima to its scores.
-                float top = reach;
+            // Half-word g of the value parameters of tokens 8 i + 2 c, 2 c + 1.
+            uint32_t w[4];
+            ldsm_x4_t(w[0], w[1], w[2], w[3], smem_u32(vb) + trans_off);
+            const uint32_t wt = max_abs<BF16>(max_abs<BF16>(w[0], w[1]), max_abs<BF16>(w[2], w[3]));
+            // max(16 s, |m|) of group g >> 1, of those (NaNs apart).
+            float top = fmaxf(fabsf(lo_f<BF16>(wt)), fabsf(hi_f<BF16>(wt))) * (lane & 4 ? 1.f : 16.f);
+            if (__any_sync(0xffffffffu, y_max > kLazyMax || top * unit > kReach)) {
+                // Rare: raise the groups' E to the value parameters of this tile, the rows' maxima to its scores.
 #pragma unroll
-                for (int sh = 1; sh <= 16; sh <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, sh));
+                for (int sh = 1; sh <= 4; sh <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, sh));
                 float drop = 1.f;  // 2^-(rise of E)
                 if (top * unit > kReach) {
                     const int old = 127 - (__float_as_int(unit) >> 23);  // E
@@ -743,6 +747,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
                     drop = exp2_int(old - en);
                     unit = exp2_int(-en);
                 }
+                float drops[kGroups];
+#pragma unroll
+                for (int j = 0; j < kGroups; ++j) drops[j] = __shfl_sync(0xffffffffu, drop, 8 * j);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -752,22 +759,23 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
                         for (int sh = 4; sh <= 16; sh <<= 1) tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, sh));
                         tm *= f_row[nt][e];
                         const float ro = r_ref[nt][e], rn = fmaxf(ro, tm == -INFINITY ? kNone : tm - kTop);
-                        const float alpha = ro == kNone ? 0.f : fast_exp2(ro - rn), alpha_v = alpha * drop;
+                        const float alpha = ro == kNone ? 0.f : fast_exp2(ro - rn);
                         r_ref[nt][e] = rn;
-                        om[nt][e] *= alpha_v;
+                        om[nt][e] *= alpha * drop;
                         om[nt][2 + e] *= alpha;
 #pragma unroll
                         for (int j = 0; j < kGroups; ++j)
 #pragma unroll
                             for (int t = 0; t < 2; ++t) {
-                                o[j][t][nt][e] *= alpha_v;
-                                o[j][t][nt][2 + e] *= alpha_v;
+                                o[j][t][nt][e] *= alpha * drops[j];
+                                o[j][t][nt][2 + e] *= alpha * drops[j];
                             }
                     }
             }
             if constexpr (EDGE) {
                 // A stored non-finite value (s = m = NaN) counts for the rows that see its token only: it
                 // becomes a NaN of their sums here, and a zero as an operand below.
+                const uint4 look = *reinterpret_cast<const uint4*>(vb + trans_off);  // of token `lane`
                 const uint32_t lw[4] = {look.x, look.y, look.z, look.w};
 #pragma unroll
                 for (int j = 0; j < kGroups; ++j) {
@@ -804,9 +812,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
                             pl[nt][i] = transpose8(lo);
                         }
                     }
-                // Half-word g of the parameters of the same tokens, times 2^-E in fp16; ones.
+                // Half-word g of their parameters, times 2^-E in fp16; ones.
                 uint32_t pt[4];
-                ldsm_x4_t(pt[0], pt[1], pt[2], pt[3], (lane & 8) ? smem_u32(sm.ones) : smem_u32(vs) + trans_off);
+                ldsm_x2_t(pt[0], pt[2], smem_u32(vs) + word_off);
+                pt[1] = pt[3] = 0x3c003c00u;
 #pragma unroll
                 for (int i = 0; i < 4; i += 2) {
                     if constexpr (EDGE) pt[i] = finite2<BF16>(pt[i]);
@@ -865,7 +874,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
 
         // ---- combine the warps' states of this item ----
         // O = 2^E (2^24 o + sum p m); n' is a sixteenth of the byte's sum less the low nibble's.
-        const float back = __int_as_float(0x7f000000 - __float_as_int(unit));  // 2^E
+        float back[kGroups];  // 2^E
+#pragma unroll
+        for (int j = 0; j < kGroups; ++j)
+            back[j] = __shfl_sync(0xffffffffu, __int_as_float(0x7f000000 - __float_as_int(unit)), 8 * j);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -875,8 +887,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
                     const float mj = __shfl_sync(0xffffffffu, om[nt][e], (2 * j + 1) * 4 + c);
 #pragma unroll
                     for (int t = 0; t < 2; ++t) {
-                        o[j][t][nt][2 + e] = fmaf(o[j][t][nt][2 + e] - o[j][t][nt][e], 1048576.f, mj) * back;
-                        o[j][t][nt][e] = fmaf(o[j][t][nt][e], 16777216.f, mj) * back;
+                        o[j][t][nt][2 + e] = fmaf(o[j][t][nt][2 + e] - o[j][t][nt][e], 1048576.f, mj) * back[j];
+                        o[j][t][nt][e] = fmaf(o[j][t][nt][e], 16777216.f, mj) * back[j];
                     }
                 }
         // Dimension of o[j][t][.][e] for e < 2; e >= 2 is the next nibble, two dimensions on.

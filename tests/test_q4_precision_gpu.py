@@ -34,6 +34,17 @@ def test_ordinary_rows(pkg, dtype, lq, hq, hkv):
     close(pkg, *make([20000, 129], hq, hkv, lq=lq, dtype=dtype, kscale=3.0, vscale=50.0, seed=hq + lq), what="peaked, split")
 
 
+@pytest.mark.parametrize("dtype,lq,hq,spread", [(BF16, 1, 4, 14), (BF16, 5, 4, 14), (BF16, 1, 4, 40), (F16, 1, 4, 11), (F16, 3, 8, 11)])
+def test_small_groups_beside_large_ones(pkg, dtype, lq, hq, spread):
+    """Groups of value dimensions 2^spread below and above their neighbours keep their own precision."""
+    q, kc, vc, cl, bt = make([900, 300], hq, 2, lq=lq, bs=128, dtype=dtype, kscale=2.0, seed=50)
+    g = torch.Generator(device="cuda").manual_seed(51)
+    x = torch.randn(vc.shape[0], 2, 128, 128, generator=g, device="cuda") + 0.2
+    for j, e in enumerate((0, -spread, spread // 2, -spread // 2)):
+        x[..., 32 * j:32 * j + 32] *= 2.0 ** e
+    close(pkg, q, kc, cache_of(x.to(dtype)), cl, bt, what=f"groups 2^{spread} apart")
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16])
 def test_small_tokens_beside_large_ones(pkg, dtype):
     """Pages whose values differ by 2^12, heads that attend to one page each."""
