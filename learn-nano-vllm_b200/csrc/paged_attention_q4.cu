@@ -16,9 +16,10 @@
 //     register both times.  For the values the second operand row is the byte n + 16 n' as it is:
 //     n' comes out by subtraction at the end, which saves a mask.  P^T turns into a B operand by
 //     movmatrix.
-//   * The words (s, m) of a token are operands too: against the rows (0, sum(q_g)), in two 16-bit
-//     parts, they give the minima's part of the score; taken to fp16 (times a power of two) and
-//     transposed, against P^T, sum_t p m, and with a row of ones beside them the softmax sum.
+//   * The words (s, m) of a token are operands too: against the rows (0, sum(q_g)), in two fp16 or
+//     three bf16 parts (22 or 24 bits), they give the minima's part of the score; taken to fp16
+//     (times a power of two) and transposed, against P^T, sum_t p m, and with a row of ones beside
+//     them the softmax sum.
 //   * The key scales multiply the products in fp32.  The value scales multiply P^T in fp16: the
 //     lanes of row 2 g of the transposed words hold them, one shuffle hands them round.
 // Roundings: p to fp16 (2^-11), the same rounded p in the products and in the sum, so that the
@@ -255,7 +256,10 @@ __device__ __forceinline__ uint32_t max_abs(uint32_t a, uint32_t b) {
     return d;
 }
 
-// Two transposed 8x8 matrices of 16-bit elements; lanes 0-15 hand their rows.
+// Two 8x8 matrices of 16-bit elements, as they lie or transposed; lanes 0-15 hand their rows.
+__device__ __forceinline__ void ldsm_x2(uint32_t& a, uint32_t& b, uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0,%1}, [%2];" : "=r"(a), "=r"(b) : "r"(addr));
+}
 __device__ __forceinline__ void ldsm_x2_t(uint32_t& a, uint32_t& b, uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0,%1}, [%2];" : "=r"(a), "=r"(b) : "r"(addr));
 }
@@ -541,12 +545,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
     const int g = lane >> 2, c = lane & 3;
     const int tok_warp = warp * kWarpTokens;
     // Byte offsets in a sub-tile's records: the rows this lane hands to ldmatrix (token lane & 7, group
-    // lane >> 3; the parameters of token lane & 15; transposed, those of token `lane` of both sub-tiles),
-    // and the parameters of token g.
+    // lane >> 3; the parameters of token `lane`, of both sub-tiles), and the parameters of token g.
     const uint32_t frag_off = uint32_t(lane & 7) * kRecord + (lane >> 3) * 16;
     const uint32_t par_off = uint32_t(g) * kRecord + q4::kParams;
-    const uint32_t word_off = uint32_t(lane & 15) * kRecord + q4::kParams;
-    const uint32_t trans_off = uint32_t(lane) * kRecord + q4::kParams;
+    const uint32_t word_off = uint32_t(lane) * kRecord + q4::kParams;
     // Scores in units of 2^-24, which the minima start as the MMAs' result; fp16 sums of q do not go down to
     // that unit, and 16 rows would spill (131.5 us against 133.4 for the verify call): there they join last.
     constexpr bool kMinFirst = BF16 && NT == 1;
@@ -558,7 +560,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
     // Query rows 8 nt + 2 c + e: reference (log2), factor of the scores.  (What the loop can recompute is not held:
     // a limit per row and the reach that E allows cost 4 us of 271, and 2 of the verify call.)
     float r_ref[NT][2], f_row[NT][2];
-    uint32_t qf[kGroups][NT][4], qs[NT][2];  // B operands of row 8 nt + g: q (two steps of a group), (0, sum q) of group c
+    // B operands of row 8 nt + g: q (two steps of a group), sum(q) of group c in parts: (0, first), (0, second),
+    // bf16 (0, first), (second, third).
+    uint32_t qf[kGroups][NT][4], qs[NT][2];
     // O^T fragments (16 dims x 8 rows in units of 2^-24), and the product with the parameter words:
     // its row g is sum_t p * (half-word g), rows 8.. are sum_t p.
     float o[kGroups][2][NT][4], om[NT][4];
@@ -617,7 +621,15 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
                     qf[j][nt][2] = pack2<false>(x[j][4], x[j][5]);
                     qf[j][nt][3] = pack2<false>(x[j][6] * 0.0625f, x[j][7] * 0.0625f);
                 }
-                split2<BF16>(make_float2(0.f, mine * (kMinFirst ? kCodeUnit : 1.f)), qs[nt][0], qs[nt][1]);
+                const float sum_q = mine * (kMinFirst ? kCodeUnit : 1.f);
+                if constexpr (BF16) {  // its 24 bits, eight at a time
+                    const float first = __uint_as_float(__float_as_uint(sum_q) & 0xffff0000u), r = sum_q - first;
+                    const float second = __uint_as_float(__float_as_uint(r) & 0xffff0000u);
+                    qs[nt][0] = __float_as_uint(first);
+                    qs[nt][1] = __byte_perm(__float_as_uint(second), __float_as_uint(r - second), 0x7632);
+                } else {
+                    split2<false>(make_float2(0.f, sum_q), qs[nt][0], qs[nt][1]);
+                }
                 // Above zero even where that underflows (all scores are 0 then): a masked -inf stays one.
                 const float fm = fmaxf(p.scale_log2 * exp2_int(eq) * (kMinFirst ? 1.f / kCodeUnit : 1.f), 1e-30f);
 #pragma unroll
@@ -678,9 +690,14 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
                 const uint4 pa4 = *reinterpret_cast<const uint4*>(ks + par_off);
                 const uint4 pb4 = *reinterpret_cast<const uint4*>(ks + par_off + 8 * kRecord);
                 const uint32_t pa[4] = {pa4.x, pa4.y, pa4.z, pa4.w}, pb[4] = {pb4.x, pb4.y, pb4.z, pb4.w};
-                uint32_t a[4];  // word c of the parameters of tokens g, g + 8, g, g + 8
+                uint32_t a[4];  // word c of the parameters of tokens g, g + 8; again, or (bf16) their minima twice
+                auto load_words = [&] {
+                    ldsm_x2(a[0], a[1], smem_u32(ks) + word_off);
+                    a[2] = BF16 ? __byte_perm(a[0], 0, 0x3232) : a[0];
+                    a[3] = BF16 ? __byte_perm(a[1], 0, 0x3232) : a[1];
+                };
                 if constexpr (kMinFirst) {
-                    ldsm_x4(a[0], a[1], a[2], a[3], smem_u32(ks) + word_off);
+                    load_words();
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) mma_zero<BF16>(x[u][nt], a, qs[nt][0], qs[nt][1]);
                 }
@@ -703,7 +720,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
                     }
                 }
                 if constexpr (!kMinFirst) {
-                    ldsm_x4(a[0], a[1], a[2], a[3], smem_u32(ks) + word_off);
+                    load_words();
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
                         float xm[4];
@@ -732,7 +749,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
                                               f_row[nt][e], -r_ref[nt][e]));
             // Half-word g of the value parameters of tokens 8 i + 2 c, 2 c + 1.
             uint32_t w[4];
-            ldsm_x4_t(w[0], w[1], w[2], w[3], smem_u32(vb) + trans_off);
+            ldsm_x4_t(w[0], w[1], w[2], w[3], smem_u32(vb) + word_off);
             const uint32_t wt = max_abs<BF16>(max_abs<BF16>(w[0], w[1]), max_abs<BF16>(w[2], w[3]));
             // max(16 s, |m|) of group g >> 1, of those (NaNs apart).
             float top = fmaxf(fabsf(lo_f<BF16>(wt)), fabsf(hi_f<BF16>(wt))) * (lane & 4 ? 1.f : 16.f);
@@ -775,7 +792,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
             if constexpr (EDGE) {
                 // A stored non-finite value (s = m = NaN) counts for the rows that see its token only: it
                 // becomes a NaN of their sums here, and a zero as an operand below.
-                const uint4 look = *reinterpret_cast<const uint4*>(vb + trans_off);  // of token `lane`
+                const uint4 look = *reinterpret_cast<const uint4*>(vb + word_off);  // of token `lane`
                 const uint32_t lw[4] = {look.x, look.y, look.z, look.w};
 #pragma unroll
                 for (int j = 0; j < kGroups; ++j) {

@@ -83,3 +83,26 @@ def test_tail_behind_one_token(pkg, dtype, n, lq, nats):
     bt = torch.arange(nb, dtype=torch.int32, device="cuda").expand(B, nb)
     cl = torch.full((B,), n, dtype=torch.int32, device="cuda")
     close(pkg, q, kc, vc, cl, bt, what=f"tail of {n}", rows=(0, 1, 37, B - 1))
+
+
+@pytest.mark.parametrize("lq", [1, 9])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_offsets_that_carry_the_scores(pkg, dtype, lq):
+    """Queries of one sign and two keys that share the weight, one an offset of the first group of dimensions
+    and one of the second (and, to even the scores, the third): minima times sums of queries are all
+    that decides, at scores of 300."""
+    B, H, bs, scale = 16, 8, 128, 0.3
+    g = torch.Generator(device="cuda").manual_seed(61)
+    q = (torch.randn(B, 1, H, 128, generator=g, device="cuda") * 1.5).exp()   # of magnitudes whose sums take many bits
+    q = q.to(dtype).expand(B, lq, H, 128).contiguous()
+    sums = q[:, 0].double().unflatten(-1, (4, 32)).sum(-1)                                 # [B, H, 4]
+    k = torch.zeros(B, H, bs, 4, dtype=torch.float64, device="cuda")
+    k[:, :, 0, 0] = (300 / scale / sums[..., 0]).to(dtype).double()
+    k[:, :, 1, 1] = (300 / scale / sums[..., 1]).to(dtype).double()
+    gap = k[:, :, 0, 0] * sums[..., 0] - k[:, :, 1, 1] * sums[..., 1]
+    k[:, :, 1, 2] = gap / sums[..., 2]
+    v = torch.zeros(B, H, bs, 128, device="cuda")
+    v[:, :, 0], v[:, :, 1] = 1, -1
+    cl = torch.full((B,), 100, dtype=torch.int32, device="cuda")
+    bt = torch.arange(B, dtype=torch.int32, device="cuda")[:, None]
+    close(pkg, q, cache_of(k.repeat_interleave(32, -1).to(dtype)), cache_of(v.to(dtype)), cl, bt, scale=scale, what="offsets")
