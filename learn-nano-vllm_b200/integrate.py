@@ -193,7 +193,7 @@ def install(fuse_qk_epilogue: bool = False, fuse_sampler: bool = False, workers:
     package's two-shot all-reduce (allreduce.AllReduce) for decode-sized outputs; it too implies
     workers.  With kv_cache_bits=4, ModelRunner.allocate_kv_cache binds 4-bit caches (quant_cache),
     3.2 times the tokens in the same memory; keys and values are quantised as they are stored.  Every
-    tensor-parallel rank must allocate the same blocks, so with several ranks it needs workers.
+    tensor-parallel rank must hold the blocks that rank 0 schedules, so it too implies workers.
     With workers, the
     engine's tensor-parallel ranks (spawned processes, nanovllm/engine/llm_engine.py:24-30)
     run install() with the same options before building their ModelRunner;
@@ -232,7 +232,7 @@ def install(fuse_qk_epilogue: bool = False, fuse_sampler: bool = False, workers:
     linear_mod.RowParallelLinear.forward = (_fused_row_parallel_forward if fuse_row_parallel else
                                             _allreduce_row_parallel_forward if row_parallel_allreduce else
                                             _ORIGINAL_ROW[0])
-    if workers or fuse_row_parallel or row_parallel_allreduce:
+    if workers or fuse_row_parallel or row_parallel_allreduce or kv_cache_bits == 4:
         import functools
         entry = importlib.import_module("__graft_entry__")
         opts = {"setup": list(worker_setup),

@@ -41,3 +41,21 @@ def test_kv_cache_bits(pkg, monkeypatch):
             pkg.install(kv_cache_bits=8)
     finally:
         integ.uninstall()
+
+
+def test_kv_cache_bits_reach_every_rank(pkg, monkeypatch):
+    """A 4-bit cache is bound in the spawned ranks too: a rank left with a 16-bit cache has fewer blocks than
+    rank 0 schedules, and its stock store writes past them."""
+    import learn_nano_vllm_b200.integrate as integ
+    for name in ("_ORIGINAL_FORWARD", "_ORIGINAL_SAMPLER", "_ORIGINAL_PREPARE", "_ORIGINAL_ROW", "_ORIGINAL_ALLOCATE"):
+        monkeypatch.setattr(integ, name, [])
+    mods, runner, original = stub_engine(monkeypatch)
+    engine = mods["nanovllm.engine.llm_engine"]
+    try:
+        pkg.install(kv_cache_bits=4)
+        assert engine.ModelRunner.func.__name__ == "nanovllm_worker"
+        assert engine.ModelRunner.keywords["options"]["install"]["kv_cache_bits"] == 4
+        pkg.install()
+        assert engine.ModelRunner is runner
+    finally:
+        integ.uninstall()
