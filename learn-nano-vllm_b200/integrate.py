@@ -134,6 +134,17 @@ def _allreduce_row_parallel_forward(self, x):
 _ORIGINAL_ALLOCATE = []
 
 
+def _least_of_ranks(blocks, world_size):
+    """The smallest count of the tensor-parallel ranks: rank 0 schedules its blocks on all of them."""
+    if world_size == 1:
+        return blocks
+    import torch.distributed as dist
+    device = torch.device("cuda", torch.cuda.current_device()) if dist.get_backend() == "nccl" else torch.device("cpu")
+    least = torch.tensor([blocks], dtype=torch.int64, device=device)
+    dist.all_reduce(least, op=dist.ReduceOp.MIN)
+    return int(least.item())
+
+
 def _q4_allocate_kv_cache(self):
     """ModelRunner.allocate_kv_cache (nanovllm/engine/model_runner.py:103-121) for 4-bit caches: the same
     share of the device memory, in blocks of 80 instead of 256 bytes per (token, kv head) and cache."""
@@ -151,7 +162,8 @@ def _q4_allocate_kv_cache(self):
     # what stays in use, and what the largest forward needed beyond it
     reserve = total - free + stats["allocated_bytes.all.peak"] - stats["allocated_bytes.all.current"]
     blocks = (int(total * cfg.gpu_memory_utilization) - reserve) // (2 * len(layers) * block)
-    cfg.num_kvcache_blocks = min(blocks, (2 ** 31 - 1) // self.block_size)  # slots are int32
+    blocks = min(blocks, (2 ** 31 - 1) // self.block_size)  # slots are int32
+    cfg.num_kvcache_blocks = _least_of_ranks(blocks, self.world_size)
     assert cfg.num_kvcache_blocks > 0, "no memory left for the KV cache"
     # zeros: records that no token was written to are finite
     self.kv_cache = torch.zeros(2, len(layers), *q4_cache_shape(cfg.num_kvcache_blocks, self.block_size, heads, head_dim),
