@@ -31,14 +31,29 @@ def set_context_source(fn):
     _get_context = fn
 
 
-# Rows of packed keys and values (8 heads: 512 bytes each) that a bound on their number may waste.
+# A bound on the rows read back serves as their number up to here (a row is Hkv * 512 bytes: 268 MB of 8 heads).
 _MAX_BOUND = 1 << 16
 
+# The last step that read its offsets: its context, the tensor and its version, the values.  A context is one
+# step's (set_context makes a new one), so the layers of a step share one read.
+_step = None
 
-def _total_bound(ctx):
-    """A host-side bound on cu_seqlens_k[-1], or None (one synchronising read) where it would be a large one."""
+
+def _offsets(ctx):
+    """cu_seqlens_k on the host: one synchronising read per step."""
+    global _step
+    cu = ctx.cu_seqlens_k
+    version = None if cu.is_inference() else cu._version
+    step = _step
+    if step is None or step[0] is not ctx or step[1] is not cu or step[2] != version:
+        step = _step = ctx, cu, version, cu.tolist()
+    return step[3]
+
+
+def _total_rows(ctx):
+    """How many rows the step's sequences are read back to: a bound while it is small, else their number."""
     bound = (ctx.cu_seqlens_k.numel() - 1) * int(ctx.max_seqlen_k)
-    return bound if bound <= _MAX_BOUND else None
+    return bound if bound <= _MAX_BOUND else _offsets(ctx)[-1]
 
 
 class Attention(nn.Module):
@@ -92,7 +107,7 @@ class Attention(nn.Module):
                                                   softmax_scale=self.scale, causal=True)
             if ctx.block_tables is not None:
                 k, v = gather_kvcache_q4(self.k_cache, self.v_cache, ctx.cu_seqlens_k, ctx.block_tables,
-                                         _total_bound(ctx), q.dtype)
+                                         _total_rows(ctx), q.dtype)
             return flash_attn_varlen_func(q, k, v, cu_seqlens_q=ctx.cu_seqlens_q, cu_seqlens_k=ctx.cu_seqlens_k,
                                           max_seqlen_q=ctx.max_seqlen_q, max_seqlen_k=ctx.max_seqlen_k,
                                           softmax_scale=self.scale, causal=True)
