@@ -31,7 +31,10 @@ def set_context_source(fn):
     _get_context = fn
 
 
-# A bound on the rows read back serves as their number up to here (a row is Hkv * 512 bytes: 268 MB of 8 heads).
+# Rows of packed keys and values that a prefill holds at a time (a row is Hkv * 512 bytes: 537 MB of 8 heads;
+# one longer sequence still makes a group of its own).  install(kv_cache_bits=4) leaves room for them.
+_PREFIX_ROWS = 1 << 17
+# A bound on the rows read back serves as their number up to here.
 _MAX_BOUND = 1 << 16
 
 # The last step that read its offsets: its context, the tensor and its version, the values.  A context is one
@@ -50,10 +53,26 @@ def _offsets(ctx):
     return step[3]
 
 
-def _total_rows(ctx):
-    """How many rows the step's sequences are read back to: a bound while it is small, else their number."""
-    bound = (ctx.cu_seqlens_k.numel() - 1) * int(ctx.max_seqlen_k)
-    return bound if bound <= _MAX_BOUND else _offsets(ctx)[-1]
+def prefix_bytes(max_model_len, num_kv_heads):
+    """Device memory that reading prefixes back may take beside a cache (head size 128, 16-bit rows)."""
+    return max(_PREFIX_ROWS, max_model_len) * num_kv_heads * 128 * 2 * 2
+
+
+def _groups(ctx):
+    """Runs of the step's sequences that are read back together: (first, last + 1, rows, longest), at most
+    _PREFIX_ROWS rows each, a bound in place of their number while it is small."""
+    n = ctx.cu_seqlens_k.numel() - 1
+    bound = n * int(ctx.max_seqlen_k)
+    if bound <= min(_MAX_BOUND, _PREFIX_ROWS):
+        return [(0, n, bound, ctx.max_seqlen_k)]
+    cu = _offsets(ctx)
+    runs, first, longest = [], 0, 0
+    for i in range(n):
+        if i > first and cu[i + 1] - cu[first] > _PREFIX_ROWS:
+            runs.append((first, i, cu[i] - cu[first], longest))
+            first, longest = i, 0
+        longest = max(longest, cu[i + 1] - cu[i])
+    return runs + [(first, n, cu[n] - cu[first], longest)]
 
 
 class Attention(nn.Module):
@@ -106,8 +125,7 @@ class Attention(nn.Module):
                                                   cache_seqlens=ctx.context_lens, block_table=ctx.block_tables,
                                                   softmax_scale=self.scale, causal=True)
             if ctx.block_tables is not None:
-                k, v = gather_kvcache_q4(self.k_cache, self.v_cache, ctx.cu_seqlens_k, ctx.block_tables,
-                                         _total_rows(ctx), q.dtype)
+                return self._attend_prefixes(ctx, q)
             return flash_attn_varlen_func(q, k, v, cu_seqlens_q=ctx.cu_seqlens_q, cu_seqlens_k=ctx.cu_seqlens_k,
                                           max_seqlen_q=ctx.max_seqlen_q, max_seqlen_k=ctx.max_seqlen_k,
                                           softmax_scale=self.scale, causal=True)
@@ -120,3 +138,18 @@ class Attention(nn.Module):
                                       cu_seqlens_q=ctx.cu_seqlens_q, cu_seqlens_k=ctx.cu_seqlens_k,
                                       max_seqlen_q=ctx.max_seqlen_q, max_seqlen_k=ctx.max_seqlen_k,
                                       softmax_scale=self.scale, causal=True, block_table=ctx.block_tables)
+
+    def _attend_prefixes(self, ctx, q):
+        """Varlen prefill over a 4-bit cache: the sequences read back as packed rows, a group at a time."""
+        groups = _groups(ctx)
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        for first, last, rows, longest in groups:
+            cu_q, cu_k, tables = ctx.cu_seqlens_q, ctx.cu_seqlens_k, ctx.block_tables
+            if len(groups) > 1:  # query offsets stay those of the whole batch, key rows start at 0
+                cu_q, cu_k, tables = cu_q[first:last + 1], cu_k[first:last + 1], tables[first:last]
+                cu_k = cu_k - cu_k[0]
+            k, v = gather_kvcache_q4(self.k_cache, self.v_cache, cu_k, tables, rows, q.dtype)
+            flash_attn_varlen_func(q, k, v, cu_seqlens_q=cu_q, cu_seqlens_k=cu_k, max_seqlen_q=ctx.max_seqlen_q,
+                                   max_seqlen_k=longest, softmax_scale=self.scale, causal=True, out=out)
+            del k, v  # before the next group's are made
+        return out

@@ -147,7 +147,8 @@ def _least_of_ranks(blocks, world_size):
 
 def _q4_allocate_kv_cache(self):
     """ModelRunner.allocate_kv_cache (nanovllm/engine/model_runner.py:103-121) for 4-bit caches: the same
-    share of the device memory, in blocks of 80 instead of 256 bytes per (token, kv head) and cache."""
+    share of the device memory, in blocks of 80 instead of 256 bytes per (token, kv head) and cache, less the
+    rows that a prefill over cached prefixes reads back."""
     from .quant_cache import q4_cache_shape
     cfg, hf = self.config, self.config.hf_config
     heads = hf.num_key_value_heads // self.world_size
@@ -159,8 +160,9 @@ def _q4_allocate_kv_cache(self):
     layers = [m for m in self.model.modules() if hasattr(m, "k_cache") and hasattr(m, "v_cache")]
     free, total = torch.cuda.mem_get_info()
     stats = torch.cuda.memory_stats()
-    # what stays in use, and what the largest forward needed beyond it
-    reserve = total - free + stats["allocated_bytes.all.peak"] - stats["allocated_bytes.all.current"]
+    # what stays in use, what the largest forward needed beyond it (without a cache), and a prefix read back
+    reserve = (total - free + stats["allocated_bytes.all.peak"] - stats["allocated_bytes.all.current"]
+               + _attention.prefix_bytes(getattr(cfg, "max_model_len", 0), heads))
     blocks = (int(total * cfg.gpu_memory_utilization) - reserve) // (2 * len(layers) * block)
     blocks = min(blocks, (2 ** 31 - 1) // self.block_size)  # slots are int32
     cfg.num_kvcache_blocks = _least_of_ranks(blocks, self.world_size)

@@ -21,7 +21,8 @@ def _worker(rank, world, port, free_blocks, ret):
         sys.path.insert(0, ROOT)
         import __graft_entry__
         pkg = __graft_entry__.load_package()
-        # a device of 1000 blocks, of which this rank finds free_blocks[rank] free
+        # a device of 1000 blocks, of which this rank finds free_blocks[rank] free; too small to read prefixes back
+        pkg.attention.prefix_bytes = lambda *a: 0
         real = torch.zeros
         torch.cuda.mem_get_info = lambda: (free_blocks[rank] * BLOCK, 1000 * BLOCK)
         torch.cuda.memory_stats = lambda: {"allocated_bytes.all.peak": 0, "allocated_bytes.all.current": 0}

@@ -80,3 +80,37 @@ def test_offsets_changed_in_place(calls):
     context.get_context().cu_seqlens_k[1:] -= 1
     a(*rows)
     assert [c[1] for c in calls if c[0] == "read"] == [70000, 69999]
+
+
+def test_rows_read_back_at_a_time_are_bounded(calls, monkeypatch):
+    """A batch of long prefixes is read back in groups of consecutive sequences; queries keep their places and
+    each group's key rows start at 0.  A sequence beyond the limit makes a group of its own."""
+    monkeypatch.setattr(mod, "_PREFIX_ROWS", 1000)
+    monkeypatch.setattr(mod, "_MAX_BOUND", 500)
+    lens_q, lens_k = [5, 7, 1, 2, 9, 3], [400, 600, 1, 2500, 300, 700]
+    rows = step(lens_q, lens_k)
+    layers(1)[0](*rows)
+    assert calls == [
+        ("read", 1000, [0, 400, 1000], [0, 1]), ("attend", [0, 5, 12], [0, 400, 1000], 600),
+        ("read", 1, [0, 1], [2]), ("attend", [12, 13], [0, 1], 1),
+        ("read", 2500, [0, 2500], [3]), ("attend", [13, 15], [0, 2500], 2500),
+        ("read", 1000, [0, 300, 1000], [4, 5]), ("attend", [15, 24, 27], [0, 300, 1000], 700)]
+
+
+def test_allocation_leaves_room(pkg, monkeypatch):
+    """The cache's share of the memory excludes the rows read back."""
+    import types
+    from learn_nano_vllm_b200 import integrate
+    block = 2 * 1 * 4 * 256 * 80
+    monkeypatch.setattr(torch.cuda, "mem_get_info", lambda: (90000 * block, 100000 * block))
+    monkeypatch.setattr(torch.cuda, "memory_stats", lambda: {"allocated_bytes.all.peak": 7 * block, "allocated_bytes.all.current": 0})
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    real = torch.zeros
+    monkeypatch.setattr(torch, "zeros", lambda *a, dtype, device: real(2, 1, *a[2:3], 1, 1, 1, dtype=dtype))
+    hf = types.SimpleNamespace(num_key_value_heads=4, num_attention_heads=8, hidden_size=1024, head_dim=128)
+    for longest in (4096, 1 << 18):
+        cfg = types.SimpleNamespace(gpu_memory_utilization=1.0, num_kvcache_blocks=-1, max_model_len=longest, hf_config=hf)
+        run = types.SimpleNamespace(config=cfg, world_size=1, block_size=256, model=torch.nn.ModuleList([mod.Attention(8, 128, 1.0, 4)]))
+        integrate._q4_allocate_kv_cache(run)
+        assert cfg.num_kvcache_blocks * block <= (90000 - 7) * block - max(1 << 17, longest) * 4 * 512
+        assert cfg.num_kvcache_blocks > 85000
