@@ -142,7 +142,9 @@ B200_API int32_t b200_gather_kvcache_q4(void* key, int64_t key_stride,
  * masks and padding rows.  The workspace works as there
  * (b200_paged_attention_q4_workspace_size bytes for the current device,
  * 256-byte aligned, zero-filled once, whatever the batch; a call leaves its
- * counters zeroed; b200_workspace_error reads its error word).  Block tables
+ * counters zeroed; b200_workspace_error reads its error word).  A call with an
+ * expired wait does too: sequences that it left unfinished and that several CTAs
+ * share come out as NaN, others keep what out held.  Block tables
  * are rows of block_table_width entries, block_table_stride apart; a tile of a
  * block id outside the cache counts as tokens of zeros.  Scores, softmax
  * statistics and sums are fp32; the probabilities p (and p * s, for the product
@@ -402,6 +404,13 @@ B200_API int32_t b200_paged_attention_noalloc_error(void* stream, int32_t* flag)
  * test check that a wait that runs out is reported to the host.
  */
 B200_API int32_t b200_testing_idle_producer(int32_t launches, int64_t wait_limit_ns);
+
+/*
+ * The same with one idle producer, that of CTA `cta` (b200_paged_attention_q4
+ * launches; in the others every producer is idle): the other CTAs do their work,
+ * the CTA's part of what it shares with them is missing.
+ */
+B200_API int32_t b200_testing_idle_cta(int32_t launches, int32_t cta, int64_t wait_limit_ns);
 
 /*
  * Causal varlen prefill attention, optionally over the paged cache (prefix

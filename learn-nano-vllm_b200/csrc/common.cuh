@@ -20,8 +20,8 @@ void clear_error();
 int device_sm_count();                                  // of the current device (cached)
 void ensure_smem_attr(const void* kernel, int bytes);   // once per kernel and device
 
-// Wait limit and idle-producer flag of the next paged attention launch on this host thread
-// (b200_testing_idle_producer; paged_attention.cu).
+// Wait limit and idle producers of the next paged attention launch on this host thread: 0 none, 1 all, 2 + n
+// that of CTA n (b200_testing_idle_producer, b200_testing_idle_cta; paged_attention.cu).
 void take_test_hook(uint64_t* wait_ns, int32_t* idle_producer);
 
 // cuTensorMapEncodeTiled for a 2-D row-major tensor [outer][inner] of 2-byte

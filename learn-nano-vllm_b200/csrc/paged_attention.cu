@@ -881,6 +881,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 // Test hook state of the calling host thread (b200_testing_idle_producer).
 thread_local int g_idle_launches = 0;
+thread_local int g_idle_cta = -1;
 thread_local uint64_t g_idle_wait_ns = kWaitLimitNs;
 
 inline void apply_test_hook(Params& prm) { take_test_hook(&prm.wait_ns, &prm.idle_producer); }
@@ -893,7 +894,7 @@ void take_test_hook(uint64_t* wait_ns, int32_t* idle_producer) {
     if (pa::g_idle_launches > 0) {
         --pa::g_idle_launches;
         *wait_ns = pa::g_idle_wait_ns;
-        *idle_producer = 1;
+        *idle_producer = pa::g_idle_cta < 0 ? 1 : 2 + pa::g_idle_cta;
     }
 }
 }  // namespace b200
@@ -905,8 +906,18 @@ extern "C" int32_t b200_testing_idle_producer(int32_t launches, int64_t wait_lim
     B200_REQUIRE(wait_limit_ns >= 1000 && wait_limit_ns <= int64_t(kWaitLimitNs),
                  "testing_idle_producer: wait limit %lld ns outside [1 us, 1 s]", (long long)wait_limit_ns);
     pa::g_idle_launches = launches;
+    pa::g_idle_cta = -1;
     pa::g_idle_wait_ns = uint64_t(wait_limit_ns);
     return B200_OK;
+}
+
+extern "C" int32_t b200_testing_idle_cta(int32_t launches, int32_t cta, int64_t wait_limit_ns) {
+    using namespace b200;
+    clear_error();
+    B200_REQUIRE(cta >= 0 && cta < (1 << 20), "testing_idle_cta: cta %d", cta);
+    const int32_t rc = b200_testing_idle_producer(launches, wait_limit_ns);
+    if (rc == B200_OK) pa::g_idle_cta = cta;
+    return rc;
 }
 
 extern "C" size_t b200_paged_attention_workspace_size(int32_t max_items, int32_t query_len, int32_t group_size,

@@ -111,7 +111,7 @@ struct Params {
     int32_t group_inv;  // ceil(2^16 / group): r / group = (r * group_inv) >> 16 for r < 16
     float scale_log2;
     uint64_t wait_ns;       // limit of every wait (kWaitLimitNs; shorter under the idle-producer test)
-    int32_t idle_producer;  // test hook: the producer issues nothing, so the consumers' first wait runs out
+    int32_t idle_producer;  // test hook: 1 every producer, 2 + n that of CTA n issues nothing, so a wait runs out
     int32_t* error;
     int32_t* counters;
     float* part_o;    // [2 * CTAs][rows][kD]
@@ -367,6 +367,30 @@ __device__ __forceinline__ void merge_share(const Params& p, const Header& hd, c
     }
 }
 
+// What this warp of a CTA with an expired wait did not finish of the pairs that the CTA shares with others: NaN
+// as its part (log_weight) and its header.  A call, and the plan made anew: inlined, or with the plan held over
+// the loop, it takes registers from the loop (3 % of a decode call).
+template <int NT>
+__device__ __noinline__ void give_up(const Params& p, Smem<NT>& sm, int warp, int lane) {
+    int length = 0, at = 0;
+    for (int b = 0; b < p.batch; ++b) length += span_of(tiles_of(sm.lens[b])) * p.hkv;
+    const int share = max(1, (length + int(gridDim.x) - 1) / int(gridDim.x));
+    const int from = int(blockIdx.x) * share;
+    for (int b = 0; b < p.batch && at < from + share; ++b) {
+        const int nt = tiles_of(sm.lens[b]), span = span_of(nt);
+        for (int h = 0; h < p.hkv && at < from + share; ++h, at += span) {
+            if (nt == 0 || at + nt <= from) continue;
+            const int first = at / share, nch = (at + nt - 1) / share - first + 1;
+            const int side = int(blockIdx.x) == first ? 1 : 0;
+            if (nch == 1 || sm.part[warp][side].nch != 0) continue;
+            __syncwarp();
+            if (lane < p.rows) p.part_lse[((2 * int64_t(blockIdx.x) + side) * kWarps + warp) * p.rows + lane] = INFINITY;
+            if (lane == 0) sm.part[warp][side] = Header{b, h, first, nch};
+            __syncwarp();
+        }
+    }
+}
+
 template <bool BF16, int NT>
 __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_kernel(const __grid_constant__ Params p) {
     using C = Cfg<NT>;
@@ -424,7 +448,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
         static_assert(kConsumers / 2 == 64, "two entries per lane");
         const int entry = __popc(__ballot_sync(0xffffffffu, sm.off[lane] * p.hkv <= begin)) +
                           __popc(__ballot_sync(0xffffffffu, sm.off[32 + lane] * p.hkv <= begin)) - 1;
-        if (lane == 0 && !p.idle_producer) {
+        if (lane == 0 && p.idle_producer != 1 && p.idle_producer != 2 + int(blockIdx.x)) {
             const uint64_t pol = l2_policy_evict_first();
             const uint32_t q_bytes = uint32_t(p.group) * kD * 2;  // one query token's rows of this kv head
             int b = 2 * entry * run, at = sm.off[entry] * p.hkv;  // `at`: where the current pair begins
@@ -983,6 +1007,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
         }
         if (!single && lane == 0) sm.part[warp][slot & 1] = hd;
     }
+
+    // A CTA with an expired wait counts all the same for the split pairs it shares, so that the counters are
+    // zero again for the next call.
+    __syncwarp();
+    if (__any_sync(0xffffffffu, *reinterpret_cast<volatile int32_t*>(&sm.err) != 0)) give_up<NT>(p, sm, warp, lane);
 
     // The run's partial items (its first and its last), after the loop so that the merge's registers are
     // not held beside it: publish this warp's share of each (one releasing count per warp, cumulative over the

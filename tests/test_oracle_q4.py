@@ -178,3 +178,10 @@ def test_c_abi_refusals(pkg):
                    (dict(kc=a + 4), ARG), (dict(ws=None), WS), (dict(ws=a + 16), WS), (dict(wb=1024), WS),
                    (dict(wb=8192), WS), (dict(b=2048, btw=1 << 22), UNS)]:
         assert lib.b200_paged_attention_q4(*{**pa, **kw}.values()) == rc, (kw, lib.b200_last_error())
+
+
+def test_idle_cta_hook_refusals(pkg):
+    lib = pkg.lib()
+    for args in ((1, -1, 2_000_000), (1, 1 << 20, 2_000_000), (-1, 0, 2_000_000), (1, 0, 10), (1, 0, 2_000_000_000)):
+        assert lib.b200_testing_idle_cta(*args) == 1, args
+    assert lib.b200_testing_idle_cta(0, 3, 2_000_000) == 0

@@ -698,3 +698,26 @@ def test_gpu_refusals(pkg):
         f(q, kc[:, :, :64].contiguous(), vc[:, :, :64].contiguous(), cache_seqlens=cl, block_table=bt)
     with pytest.raises(AssertionError):
         f(q.transpose(2, 3).contiguous().transpose(2, 3), kc, vc, cache_seqlens=cl, block_table=bt)
+
+
+@pytest.mark.parametrize("ctx,hq,hkv,lq,cta", [([20000, 300], 8, 2, 1, 3), ([57000], 4, 1, 1, 40), ([57000], 4, 1, 1, 0), ([9000, 1, 16500], 8, 1, 1, 7),
+                                               ([33000, 100, 9000], 4, 2, 5, 20), ([2000] * 150, 16, 8, 1, 5)])
+def test_a_stalled_cta_leaves_its_workspace_usable(pkg, ctx, hq, hkv, lq, cta):
+    """One CTA's producer issues nothing (test hook): the call reports it, what the CTA shares with others comes out as
+    NaN, the counters are zero again, and the next call on the workspace, of other queries, is right."""
+    q, kc, vc, cl, bt = make(ctx, hq, hkv, lq=lq, seed=sum(ctx) + cta)
+    ws = torch.zeros(pkg.q4_workspace_size(lq, hq // hkv), dtype=torch.uint8, device="cuda")
+    f = lambda x: pkg.flash_attn_with_kvcache_q4(x, kc, vc, cache_seqlens=cl, block_table=bt, workspace=ws, out=torch.zeros_like(x))
+    want = f(q)
+    assert pkg.workspace_error(ws) == 0 and torch.isfinite(want).all()
+    assert pkg.lib().b200_testing_idle_cta(1, cta, 2_000_000) == 0
+    stalled = f(q)
+    assert pkg.workspace_error(ws) & 1
+    assert int(ws[256:7424].view(torch.int32).abs().sum()) == 0
+    hit = torch.isnan(stalled)
+    assert hit.any() and not hit.all() or len(ctx) == 1
+    same = ~hit & (stalled != 0)   # what no stalled CTA touched
+    assert torch.equal(stalled[same], want[same])
+    got = f(-q)
+    ws.zero_()
+    assert torch.equal(got, f(-q)) and pkg.workspace_error(ws) == 0
