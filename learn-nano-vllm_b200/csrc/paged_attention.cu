@@ -872,7 +872,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         __threadfence();
         const int done = atomicAdd(&p.ctrl[1], 1);
         if (done == int(gridDim.x) - 1) {
-            // Every CTA has stopped claiming items: re-arm the scheduler.
+            // Every CTA has stopped claiming items: re-arm the scheduler, and the split counters where a
+            // CTA with an expired wait may have left some without an arrival.
+            if (atomicOr(&p.ctrl[2], 0) != 0)
+                for (int i = 0; i < p.batch * p.hkv; ++i) p.counters[i] = 0;
             atomicExch(&p.ctrl[0], 0);
             atomicExch(&p.ctrl[1], 0);
         }

@@ -205,3 +205,22 @@ def test_wait_that_runs_out_is_reported(pkg):
     assert pkg.workspace_error(ws) == 0
     want = oatt.paged_attention_ref(host(q), host(kc), host(vc), case.block_tables, case.context_lens, case.scale)
     assert_attn_close(host(out), want, "after the stalled call")
+
+
+def test_lost_arrivals_do_not_outlive_their_call(pkg):
+    """The state that a CTA with an expired wait leaves (error word set, split counters off) is gone after that call:
+    the next one on the workspace, of other queries, is right."""
+    lib = pkg.lib()
+    case = cases.make_paged_case([30000, 17, 9000], 16, 8, lq=1, seed=4)
+    q, kc, vc = dev_bf16(case.q), dev_bf16(case.k_cache), dev_bf16(case.v_cache)
+    cl, bt = dev_i32(case.context_lens), dev_i32(case.block_tables)
+    ws = torch.zeros(lib.b200_paged_attention_workspace_size(4096, 1, 2, 128), dtype=torch.uint8, device="cuda")
+    want = [pkg.paged_attention(x, kc, vc, cl, bt, case.scale, workspace=ws).clone() for x in (q, -q)]
+    words = ws.view(torch.int32)
+    assert int(words[:64 + 3 * 8].abs().sum()) == 0
+    words[2] = 1
+    words[64:64 + 3 * 8] = 1000      # no pair has as many chunks: none is merged in this call
+    pkg.paged_attention(q, kc, vc, cl, bt, case.scale, workspace=ws)
+    assert int(words[64:64 + 3 * 8].abs().sum()) == 0 and pkg.workspace_error(ws) == 1
+    for x, w in zip((-q, q), want[::-1]):
+        assert torch.equal(pkg.paged_attention(x, kc, vc, cl, bt, case.scale, workspace=ws), w)
