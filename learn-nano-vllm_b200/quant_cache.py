@@ -30,8 +30,9 @@ HEAD_DIM = 128
 RECORD_BYTES = 80
 _CONTROL_BYTES = 16384  # covers the control words and counters at the start of an attention workspace
 _U8, _I32 = torch.uint8, torch.int32
-_current_device = torch._C._cuda_getDevice
-_raw_stream = torch._C._cuda_getCurrentRawStream  # the handle that torch.cuda.current_stream wraps
+# A torch without CUDA has neither; no call gets as far without a CUDA tensor.
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # the handle that torch.cuda.current_stream wraps
 
 
 def q4_cache_shape(num_blocks: int, block_size: int, num_kv_heads: int, head_dim: int = HEAD_DIM) -> tuple:

@@ -185,3 +185,20 @@ def test_idle_cta_hook_refusals(pkg):
     for args in ((1, -1, 2_000_000), (1, 1 << 20, 2_000_000), (-1, 0, 2_000_000), (1, 0, 10), (1, 0, 2_000_000_000)):
         assert lib.b200_testing_idle_cta(*args) == 1, args
     assert lib.b200_testing_idle_cta(0, 3, 2_000_000) == 0
+
+
+def test_import_without_a_cuda_build_of_torch():
+    """The package imports where torch has no CUDA bindings; CUDA tensors, which the ops ask for, do not exist there."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    code = ("import torch\n"
+            "for n in [n for n in dir(torch._C) if n.startswith('_cuda_get')]: delattr(torch._C, n)\n"
+            "import __graft_entry__\n"
+            "pkg = __graft_entry__.load_package()\n"
+            "k, c = torch.zeros(1, 1, 128, dtype=torch.bfloat16), torch.zeros(1, 1, 128, 80, dtype=torch.uint8)\n"
+            "try: pkg.store_kvcache_q4(k, k, c, c, torch.zeros(1, dtype=torch.int32))\n"
+            "except AssertionError as e: print('refused', e)\n")
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "refused 4-bit KV cache ops take CUDA tensors" in r.stdout, r.stderr
