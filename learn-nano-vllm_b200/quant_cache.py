@@ -270,7 +270,7 @@ def flash_attn_with_kvcache_q4(q, k_cache, v_cache, cache_seqlens=None, block_ta
     cache_seqlens int32 [B] counts the cached tokens of each row including its Lq queries; rows
     with cache_seqlens <= 0 return zeros.  Tokens whose page lies outside the cache count as zeros.
     workspace: a caller-owned one of q4_workspace_size(Lq, Hq // Hkv) bytes, zero-filled
-    once; calls that share it must not overlap (default: one per stream, or per captured call).
+    once; calls that share it must not overlap (default: one per stream, or per captured graph and stream).
     """
     assert cache_seqlens is not None and block_table is not None, "the B200 path reads a paged cache"
     shape, qs, cs, bt = q.shape, q.stride(), k_cache.shape, block_table.shape
