@@ -37,19 +37,20 @@ _PREFIX_ROWS = 1 << 17
 # A bound on the rows read back serves as their number up to here.
 _MAX_BOUND = 1 << 16
 
-# The last step that read its offsets: its context, the tensor and its version, the values.  A context is one
-# step's (set_context makes a new one), so the layers of a step share one read.
+# The last step that read its offsets: its context, the tensor and its version, the values, the layers served.
 _step = None
 
 
-def _offsets(ctx):
-    """cu_seqlens_k on the host: one synchronising read per step."""
+def _offsets(ctx, layer):
+    """cu_seqlens_k on the host: one synchronising read per step, shared by the step's layers through its context.
+    A layer that comes by again is in another step (its lengths may have been written in place)."""
     global _step
     cu = ctx.cu_seqlens_k
     version = None if cu.is_inference() else cu._version
     step = _step
-    if step is None or step[0] is not ctx or step[1] is not cu or step[2] != version:
-        step = _step = ctx, cu, version, cu.tolist()
+    if step is None or step[0] is not ctx or step[1] is not cu or step[2] != version or id(layer) in step[4]:
+        step = _step = ctx, cu, version, cu.tolist(), set()
+    step[4].add(id(layer))
     return step[3]
 
 
@@ -58,14 +59,14 @@ def prefix_bytes(max_model_len, num_kv_heads):
     return max(_PREFIX_ROWS, max_model_len) * num_kv_heads * 128 * 2 * 2
 
 
-def _groups(ctx):
+def _groups(ctx, layer):
     """Runs of the step's sequences that are read back together: (first, last + 1, rows, longest), at most
     _PREFIX_ROWS rows each, a bound in place of their number while it is small."""
     n = ctx.cu_seqlens_k.numel() - 1
     bound = n * int(ctx.max_seqlen_k)
     if bound <= min(_MAX_BOUND, _PREFIX_ROWS):
         return [(0, n, bound, ctx.max_seqlen_k)]
-    cu = _offsets(ctx)
+    cu = _offsets(ctx, layer)
     runs, first, longest = [], 0, 0
     for i in range(n):
         if i > first and cu[i + 1] - cu[first] > _PREFIX_ROWS:
@@ -141,7 +142,7 @@ class Attention(nn.Module):
 
     def _attend_prefixes(self, ctx, q):
         """Varlen prefill over a 4-bit cache: the sequences read back as packed rows, a group at a time."""
-        groups = _groups(ctx)
+        groups = _groups(ctx, self)
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         for first, last, rows, longest in groups:
             cu_q, cu_k, tables = ctx.cu_seqlens_q, ctx.cu_seqlens_k, ctx.block_tables

@@ -114,3 +114,15 @@ def test_allocation_leaves_room(pkg, monkeypatch):
         integrate._q4_allocate_kv_cache(run)
         assert cfg.num_kvcache_blocks * block <= (90000 - 7) * block - max(1 << 17, longest) * 4 * 512
         assert cfg.num_kvcache_blocks > 85000
+
+
+def test_a_context_used_for_several_steps(calls):
+    """Lengths written in place under one context, in inference mode (no version counts there): each step reads its own."""
+    with torch.inference_mode():
+        rows = step([1] * 70, [1000] * 70)
+        ls = layers(2)
+        for taken in (0, 1, 5):
+            context.get_context().cu_seqlens_k[1:] -= taken
+            for a in ls:
+                a(*rows)
+    assert [c[1] for c in calls if c[0] == "read"] == [70000] * 2 + [69999] * 2 + [69994] * 2
