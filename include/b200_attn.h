@@ -94,7 +94,8 @@ B200_API int32_t b200_store_kvcache(const void* key, int64_t key_stride,
  * holds dimensions 8w .. 8w + 7: nibbles 0-3 the even ones, 4-7 the odd ones.
  *     m = min x, s = (max x - m) / 15 in fp32 rounded to dtype (0 if < 2^-100),
  *     code = min(15, rint((x - m) / s)), value = s * code + m (read back rounded once to dtype);
- * a group whose max - min is not finite gets s = m = NaN, codes 0.  A cache is
+ * a group whose max - min is not finite gets s = m = NaN, codes 0; where s * 15 + m
+ * passes dtype's largest number (s is rounded), code 15 reads back as an infinity.  A cache is
  * read with the dtype it was written with.  head_dim is 128.
  *
  * store: quantises key / value rows [num_tokens, Hkv, 128] into the records of

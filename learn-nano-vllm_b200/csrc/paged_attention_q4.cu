@@ -25,7 +25,8 @@
 // Roundings: p to fp16 (2^-11), the same rounded p in the products and in the sum, so that the
 // result is a mean under weights off by as much; p s to fp16 (2^-11).  fp16 models, whose outputs
 // would show both, carry the rest of p and of p s in a second product (0.00023 from 64 bits
-// relative, 0.00034 without; the output's own rounding is 0.0002).  Sums and maxima are fp32.
+// relative, 0.00034 without; the output's own rounding is 0.0002).  Sums and maxima are fp32, but
+// for what a matrix product cuts (above).
 //
 // Ranges.  p = 2^(x - r) with r lazily raised to 2^8 below the running maximum, so p <= 2^kLazyMax.  The
 // value parameters enter as 2^-E of themselves, one E per group, which follows the group's largest
@@ -49,8 +50,8 @@
 // bounded (kWaitLimitNs, or the test limit).
 //
 // What bounds it (512 sequences, 1.17 M tokens, 8 kv heads of 4 rows: 1.50 GB, 228 us at the measured
-// copy rate): 267 us, 157 M warp instructions, the vector pipes; held for a second it reaches the
-// board's power cap, 1.74 GHz and 290 to 313 us.  A record costs its share of 268 instructions per
+// copy rate): 267 us, 158 M warp instructions, the vector pipes; held for a second it reaches the
+// board's power cap, 1.69 GHz and 310 to 313 us.  A record costs its share of 271 instructions per
 // 16 tokens, 72 of them masks.  16 consumer warps per SM (104 registers each, taken from their
 // producers) issue more often, spill, and gain nothing; they would cost the short calls 2 us.
 #include <atomic>
