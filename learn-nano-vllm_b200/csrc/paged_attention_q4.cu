@@ -219,13 +219,11 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 
 __device__ __forceinline__ float exp2_int(int e) { return __int_as_float((127 + e) << 23); }  // -126 <= e <= 127
 
-// Two 16-bit parts of a pair of floats: hi + lo = x to 16 (bf16) or 22 (fp16) bits.
-template <bool BF16>
+// Two fp16 parts of a pair of floats: hi + lo = x to 22 bits.
 __device__ __forceinline__ void split2(float2 x, uint32_t& hi, uint32_t& lo) {
-    if constexpr (BF16) hi = __byte_perm(__float_as_uint(x.x), __float_as_uint(x.y), 0x7632);  // truncated
-    else hi = pack2<false>(x.x, x.y);
-    const float2 r = fsub2(x, make_float2(lo_f<BF16>(hi), hi_f<BF16>(hi)));
-    lo = pack2<BF16>(r.x, r.y);
+    hi = pack2<false>(x.x, x.y);
+    const float2 r = fsub2(x, make_float2(lo_f<false>(hi), hi_f<false>(hi)));
+    lo = pack2<false>(r.x, r.y);
 }
 
 // A pair of 16-bit floats with its infinities and NaNs replaced by zeros.
@@ -653,7 +651,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
                     qs[nt][0] = __float_as_uint(first);
                     qs[nt][1] = __byte_perm(__float_as_uint(second), __float_as_uint(r - second), 0x7632);
                 } else {
-                    split2<false>(make_float2(0.f, sum_q), qs[nt][0], qs[nt][1]);
+                    split2(make_float2(0.f, sum_q), qs[nt][0], qs[nt][1]);
                 }
                 // Above zero even where that underflows (all scores are 0 then): a masked -inf stays one.
                 const float fm = fmaxf(p.scale_log2 * exp2_int(eq) * (kMinFirst ? 1.f / kCodeUnit : 1.f), 1e-30f);
@@ -859,7 +857,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::kCtas) paged_attention_q4_k
                             pb[nt][i] = transpose8(pack2<false>(y.x, y.y));
                         } else {
                             uint32_t hi, lo;
-                            split2<false>(y, hi, lo);
+                            split2(y, hi, lo);
                             pb[nt][i] = transpose8(hi);
                             pl[nt][i] = transpose8(lo);
                         }
